@@ -23,13 +23,14 @@ LIB_PATH = os.path.join(LIB_DIR, "libmantle_cuda_sampler.so")
 NCCL_LIB_PATH = os.path.join(LIB_DIR, "libmantle_cuda_sampler_nccl.so")
 NCCL_SOURCES = ["sharded_nccl.cu"]
 
-SOURCES = ["sampler_kernels.cu", "host_sampler.cu", "host_batch_sampler.cu"]
+SOURCES = ["sampler_kernels.cu", "host_sampler.cu", "host_batch_sampler.cu", "head_kernels.cu"]
 HEADERS = [
     os.path.join(ROOT, "include", "mantle_cuda_sampler.h"),
     os.path.join(ROOT, "include", "mantle_sample_params.h"),
     os.path.join(ROOT, "include", "mantle_host_sampler.h"),
     os.path.join(ROOT, "include", "mantle_batch_sampler.h"),
     os.path.join(ROOT, "include", "mantle_cuda_sampler_nccl.h"),
+    os.path.join(ROOT, "include", "mantle_head.h"),
 ]
 
 NVCC_FLAGS = [

@@ -1,0 +1,274 @@
+// What the head projection needs to know about a batch's adapters, worked out on the device: which rows
+// use which adapter, and each row's rank-long product with its adapter's first factor.
+// Part of head_kernels.cu.
+//
+// The projection (head_rows.cuh) adds an adapter to a tile of rows as a few more steps of its matrix product:
+//
+//     D[v][row] += sum_j B[a][v][j] * u[row][j],     u[row][j] = gain[a] * sum_k x^[row][k] A[a][j][k]
+//
+// for the rows that use adapter a.  For that the rows are put in an order in which those of one adapter
+// stand together (head_sort_kernel), so that such a step covers a window of neighbouring columns of D and
+// not the whole tile; u is laid out per window with zeros for the columns that belong to other rows
+// (head_shrink_kernel), which makes the windows' products plain sums.  A row's result does not depend on
+// where in the order it stands: a column of D only ever sees its own column of the operands.
+#pragma once
+
+namespace {
+
+constexpr int U_CHUNK = 32;        // ranks of one step: a row of u holds 32 leading parts and 32 remainders
+constexpr int U_ROW = 2 * U_CHUNK; // bfloat16 elements, 128 bytes
+constexpr int WINDOW = 16;         // columns of D come in sixteens
+constexpr int SLOT_COLS = 128;     // a slot's window lies within an aligned run of 128 columns of its tile
+constexpr int SORT_NT = 1024;
+
+// One step's worth of columns: adapter `adapter` on columns [col, col + n) of its row tile, with the rows of u
+// from u_row on.  16 bytes, read as one int4.
+struct HeadSlot {
+    int adapter, col, n, u_row;
+};
+// Sixteen rows of u: sorted places [place, place + 16), of which [first, last) use the adapter.
+struct HeadBox {
+    int adapter, place, first, last;
+};
+
+struct HeadPrep {
+    // in
+    const void* x;
+    const float* x_scales;
+    const bf16_raw* a;
+    const float* gain;
+    const int32_t* ids;
+    long long x_stride;  // elements
+    int rows, hidden, e4m3, vec;  // vec: rows of x start on 16 bytes
+    int n_adapters, rank, chunks;
+    int tile_cols, row_tiles;
+    int box_bound, copy_ctas;
+    // workspace
+    int* perm;        // [rows] sorted place -> row
+    HeadSlot* slots;
+    HeadBox* boxes;
+    int* tile_first;  // [row_tiles + 1] first slot of a tile
+    int* n_boxes;     // [1]
+    bf16_raw* u;      // [chunks][16 * box_bound][U_ROW]
+    void* xs;         // [rows][hidden] sorted, contiguous
+};
+
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+// Exclusive sum of `v` over the CTA's threads; *total gets the whole.
+__device__ __forceinline__ int block_scan(int v, int* warp_sums, int* total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int s = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int w = __shfl_up_sync(0xffffffffu, s, o);
+        if (lane >= o) s += w;
+    }
+    __syncthreads();  // warp_sums may still be read from the call before
+    if (lane == 31) warp_sums[warp] = s;
+    __syncthreads();
+    int w = warp_sums[lane];  // SORT_NT / 32 = 32 of them
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, w, o);
+        if (lane >= o) w += x;
+    }
+    *total = __shfl_sync(0xffffffffu, w, 31);
+    const int before = warp ? __shfl_sync(0xffffffffu, w, warp - 1) : 0;
+    return before + s - v;
+}
+
+// One CTA: counts the rows of every adapter, gives each adapter its run of places (rows without one come
+// last), and cuts the runs into slots and boxes.  Shared memory: n_adapters + 1 counts.
+__global__ void __launch_bounds__(SORT_NT) head_sort_kernel(const HeadPrep p) {
+    extern __shared__ int bins[];  // [n_adapters + 1]: counts, then next free places, then ends of runs
+    __shared__ int warp_sums[32];
+    pdl_trigger();
+    const int n = p.n_adapters, tid = threadIdx.x;
+    for (int b = tid; b <= n; b += SORT_NT) bins[b] = 0;
+    __syncthreads();
+    for (int r = tid; r < p.rows; r += SORT_NT) {
+        const int id = p.ids[r];
+        atomicAdd(&bins[id >= 0 && id < n ? id : n], 1);
+    }
+    __syncthreads();
+    int carry = 0;
+    for (int b0 = 0; b0 <= n; b0 += SORT_NT) {
+        const int b = b0 + tid, v = b <= n ? bins[b] : 0;
+        int total;
+        const int at = carry + block_scan(v, warp_sums, &total);
+        if (b <= n) bins[b] = at;
+        carry += total;
+    }
+    __syncthreads();
+    for (int r = tid; r < p.rows; r += SORT_NT) {
+        const int id = p.ids[r];
+        p.perm[atomicAdd(&bins[id >= 0 && id < n ? id : n], 1)] = r;
+    }
+    __syncthreads();  // bins[b] is now the end of run b, and its start the end of run b - 1
+
+    // A run is cut where a tile ends, and inside a tile at every 128 columns.
+    int slot_carry = 0, box_carry = 0;
+    for (int b0 = 0; b0 < n; b0 += SORT_NT) {
+        const int b = b0 + tid;
+        const int lo = b < n ? (b ? bins[b - 1] : 0) : 0, hi = b < n ? bins[b] : 0;
+        auto cut = [&](int at) {  // end of the piece that starts at place `at`
+            const int tile = at / p.tile_cols, col = at % p.tile_cols;
+            return min(hi, min((tile + 1) * p.tile_cols, tile * p.tile_cols + (col / SLOT_COLS + 1) * SLOT_COLS));
+        };
+        int n_slots = 0, n_boxes = 0;
+        for (int at = lo; at < hi;) {
+            const int end = cut(at), tile0 = at / p.tile_cols * p.tile_cols;
+            const int c0 = (at - tile0) / WINDOW, c1 = (end - tile0 + WINDOW - 1) / WINDOW;
+            n_slots++;
+            n_boxes += c1 - c0;
+            at = end;
+        }
+        int slot_total, box_total;
+        int slot = slot_carry + block_scan(n_slots, warp_sums, &slot_total);
+        int box = box_carry + block_scan(n_boxes, warp_sums, &box_total);
+        for (int at = lo; at < hi;) {
+            const int end = cut(at), tile = at / p.tile_cols, tile0 = tile * p.tile_cols;
+            const int c0 = (at - tile0) / WINDOW, c1 = (end - tile0 + WINDOW - 1) / WINDOW;
+            HeadSlot s = {b, c0 * WINDOW, (c1 - c0) * WINDOW, box * WINDOW};
+            p.slots[slot] = s;
+            // the first slot of a tile is the one whose predecessor -- the place before it, if that has an adapter --
+            // lies in another tile; rows with adapters are gapless from place 0 on
+            if (at == tile0) p.tile_first[tile] = slot;
+            for (int c = c0; c < c1; c++) {
+                HeadBox x = {b, tile0 + c * WINDOW, at, end};
+                p.boxes[box++] = x;
+            }
+            slot++;
+            at = end;
+        }
+        slot_carry += slot_total;
+        box_carry += box_total;
+    }
+    // tiles from the first place without an adapter on that no slot starts: empty
+    __syncthreads();
+    const int with = n ? bins[n - 1] : 0;
+    const int last_tile = (with + p.tile_cols - 1) / p.tile_cols;
+    for (int t = last_tile + tid; t <= p.row_tiles; t += SORT_NT) p.tile_first[t] = slot_carry;
+    if (tid == 0) *p.n_boxes = box_carry;
+}
+
+__device__ __forceinline__ void mma_16x8x16(float d[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                            uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// two e4m3 (exact in f16, and from there in bfloat16) to two bfloat16
+__device__ __forceinline__ uint32_t e4m3x2_to_bf16x2(uint32_t two) {
+    uint32_t h;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)two));
+    float lo, hi;
+    asm("{.reg .b16 l, u; mov.b32 {l, u}, %2; cvt.f32.f16 %0, l; cvt.f32.f16 %1, u;}" : "=f"(lo), "=f"(hi) : "r"(h));
+    return pack_bf16(lo, hi);
+}
+
+// Eight neighbouring values of one row of x as four bfloat16 pairs.
+__device__ __forceinline__ uint4 x_eight(const HeadPrep& p, const char* row, int k) {
+    if (p.e4m3) {
+        uint32_t w[2];
+        if (p.vec) {
+            const uint2 u = *reinterpret_cast<const uint2*>(row + k);
+            w[0] = u.x, w[1] = u.y;
+        } else {
+            const uint8_t* q = reinterpret_cast<const uint8_t*>(row) + k;
+#pragma unroll
+            for (int i = 0; i < 2; i++) w[i] = q[4 * i] | q[4 * i + 1] << 8 | q[4 * i + 2] << 16 | (uint32_t)q[4 * i + 3] << 24;
+        }
+        return make_uint4(e4m3x2_to_bf16x2(w[0] & 0xffff), e4m3x2_to_bf16x2(w[0] >> 16), e4m3x2_to_bf16x2(w[1] & 0xffff),
+                          e4m3x2_to_bf16x2(w[1] >> 16));
+    }
+    const bf16_raw* q = reinterpret_cast<const bf16_raw*>(row) + k;
+    if (p.vec) return *reinterpret_cast<const uint4*>(q);
+    return make_uint4(q[0] | (uint32_t)q[1] << 16, q[2] | (uint32_t)q[3] << 16, q[4] | (uint32_t)q[5] << 16,
+                      q[6] | (uint32_t)q[7] << 16);
+}
+
+// CTAs [0, box_bound) x [0, rank / 8): eight ranks of sixteen rows of u.  The warps share out the columns of x
+// and add their sums up in shared memory.  The order of the columns within a step is free in a dot product, so
+// each lane takes eight neighbours of its row, one 16-byte load, as two steps' operands.
+// CTAs from box_bound on (blockIdx.y 0): the sorted copy of x.
+__global__ void __launch_bounds__(256) head_shrink_kernel(const HeadPrep p) {
+    __shared__ float sums[8][16][8];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int esz = p.e4m3 ? 1 : 2;
+    pdl_trigger();
+    pdl_wait();
+    if ((int)blockIdx.x >= p.box_bound) {
+        if (blockIdx.y) return;
+        const int w0 = ((int)blockIdx.x - p.box_bound) * 8 + warp;
+        const long long bytes = (long long)p.hidden * esz;  // a multiple of 16
+        for (int r = w0; r < p.rows; r += p.copy_ctas * 8) {
+            const int from = p.n_adapters ? p.perm[r] : r;
+            const char* src = static_cast<const char*>(p.x) + (long long)from * p.x_stride * esz;
+            char* dst = static_cast<char*>(p.xs) + r * bytes;
+            if (p.vec) {
+                for (long long i = lane * 16; i < bytes; i += 512) *reinterpret_cast<uint4*>(dst + i) = *reinterpret_cast<const uint4*>(src + i);
+            } else if (p.e4m3) {
+                for (long long i = lane; i < bytes; i += 32) dst[i] = src[i];
+            } else {
+                for (long long i = lane * 2; i < bytes; i += 64) *reinterpret_cast<bf16_raw*>(dst + i) = *reinterpret_cast<const bf16_raw*>(src + i);
+            }
+        }
+        return;
+    }
+    if ((int)blockIdx.x >= *p.n_boxes) return;
+    const HeadBox box = p.boxes[blockIdx.x];
+    const int adapter = box.adapter, place = box.place, first = box.first, last = box.last;
+    const int j0 = blockIdx.y * 8;
+    const int g = lane >> 2, q = lane & 3;
+    // the two rows of x this lane loads from (null: zeros), and its row of A
+    const char* row[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const int at = place + g + 8 * i;
+        row[i] = at >= first && at < last ? static_cast<const char*>(p.x) + (long long)p.perm[at] * p.x_stride * esz : nullptr;
+    }
+    const bf16_raw* arow = p.a + ((long long)adapter * p.rank + j0 + g) * p.hidden;
+    float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    const uint4 none = make_uint4(0, 0, 0, 0);
+#pragma unroll 4
+    for (int k = warp * 32 + q * 8; k < p.hidden + q * 8; k += 256) {  // the same count for a warp's lanes
+        const bool in = k < p.hidden;
+        const uint4 b = in ? *reinterpret_cast<const uint4*>(arow + k) : none;
+        const uint4 x0 = in && row[0] ? x_eight(p, row[0], k) : none;
+        const uint4 x1 = in && row[1] ? x_eight(p, row[1], k) : none;
+        mma_16x8x16(d, x0.x, x1.x, x0.y, x1.y, b.x, b.y);
+        mma_16x8x16(d, x0.z, x1.z, x0.w, x1.w, b.z, b.w);
+    }
+    sums[warp][g][q * 2] = d[0], sums[warp][g][q * 2 + 1] = d[1];
+    sums[warp][g + 8][q * 2] = d[2], sums[warp][g + 8][q * 2 + 1] = d[3];
+    __syncthreads();
+    if (threadIdx.x >= 128) return;
+    const int i = threadIdx.x >> 3, j = threadIdx.x & 7, at = place + i;
+    float v = 0.0f;
+    if (at >= first && at < last) {
+#pragma unroll
+        for (int w = 0; w < 8; w++) v += sums[w][i][j];
+        if (p.gain) v *= p.gain[adapter];
+        if (p.e4m3) v *= p.x_scales[p.perm[at]];
+    }
+    // v in two bfloat16: 16 bits of mantissa (an infinity or NaN stays in the leading part alone)
+    const uint32_t hi = pack_bf16(v, 0.0f) & 0xffffu;
+    const float rest = v - __uint_as_float(hi << 16);
+    const uint32_t lo = (hi & 0x7f80u) == 0x7f80u ? 0u : pack_bf16(rest, 0.0f) & 0xffffu;
+    const int rank_at = j0 + j, chunk = rank_at / U_CHUNK;
+    bf16_raw* u = p.u + (((long long)chunk * p.box_bound + blockIdx.x) * WINDOW + i) * U_ROW + rank_at % U_CHUNK;
+    u[0] = (bf16_raw)hi;
+    u[U_CHUNK] = (bf16_raw)lo;
+    // a rank that ends inside a step of sixteen: zeros up to its end
+    if (rank_at + 8 >= p.rank && p.rank % 16) {
+        u[8] = 0;
+        u[U_CHUNK + 8] = 0;
+    }
+}
+
+}  // namespace

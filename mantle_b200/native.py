@@ -12,6 +12,7 @@ from . import build as _build
 
 DTYPE_F32 = 0
 DTYPE_BF16 = 1
+DTYPE_E4M3 = 2
 MAX_TOP_K = 1024
 MAX_VOCAB = 1 << 20
 FLAG_WRITE_BACK_PENALTY = 1
@@ -72,6 +73,62 @@ class SampleBatch(C.Structure):
         ("token_prob", C.c_void_p),
         ("softmax_sum", C.c_void_p),
         ("skip", C.c_void_p),
+    ]
+
+
+class NormBatch(C.Structure):
+    """MantleNormBatch, include/mantle_head.h."""
+
+    _fields_ = [
+        ("x", C.c_void_p),
+        ("residual", C.c_void_p),
+        ("residual_out", C.c_void_p),
+        ("weight", C.c_void_p),
+        ("out", C.c_void_p),
+        ("out_scale", C.c_void_p),
+        ("x_stride", C.c_int64),
+        ("residual_stride", C.c_int64),
+        ("residual_out_stride", C.c_int64),
+        ("out_stride", C.c_int64),
+        ("scale_stride", C.c_int64),
+        ("rows", C.c_int32),
+        ("hidden", C.c_int32),
+        ("dtype", C.c_int32),
+        ("weight_dtype", C.c_int32),
+        ("out_dtype", C.c_int32),
+        ("scale_group", C.c_int32),
+        ("eps", C.c_float),
+        ("weight_offset", C.c_float),
+    ]
+
+
+class HeadBatch(C.Structure):
+    """MantleHeadBatch, include/mantle_head.h."""
+
+    _fields_ = [
+        ("hidden_rows", C.c_void_p),
+        ("weight", C.c_void_p),
+        ("base", C.c_void_p),
+        ("hidden_scales", C.c_void_p),
+        ("weight_scales", C.c_void_p),
+        ("adapter_a", C.c_void_p),
+        ("adapter_b", C.c_void_p),
+        ("adapter_gain", C.c_void_p),
+        ("adapter_ids", C.c_void_p),
+        ("out", C.c_void_p),
+        ("status", C.c_void_p),
+        ("hidden_stride", C.c_int64),
+        ("weight_stride", C.c_int64),
+        ("base_stride", C.c_int64),
+        ("out_stride", C.c_int64),
+        ("rows", C.c_int32),
+        ("vocab", C.c_int32),
+        ("hidden", C.c_int32),
+        ("dtype", C.c_int32),
+        ("out_dtype", C.c_int32),
+        ("n_adapters", C.c_int32),
+        ("rank", C.c_int32),
+        ("reserved", C.c_int32),
     ]
 
 
@@ -157,6 +214,14 @@ BATCH_EXPORTS = {
         C.c_int, [C.c_void_p, C.POINTER(C.c_void_p), C.POINTER(C.c_void_p), C.POINTER(C.c_int32), C.POINTER(C.c_void_p)]),
 }
 
+# include/mantle_head.h
+HEAD_EXPORTS = {
+    "mantleCudaNormRows": (C.c_int, [C.POINTER(NormBatch), C.c_void_p]),
+    "mantleCudaHeadRows": (C.c_int, [C.POINTER(HeadBatch), C.c_void_p, C.c_size_t, C.c_void_p]),
+    "mantleCudaHeadWorkspaceBytes": (C.c_int, [C.POINTER(HeadBatch), C.POINTER(C.c_size_t)]),
+    "mantleCudaHeadLaunches": (C.c_int, [C.POINTER(HeadBatch), C.POINTER(C.c_int)]),
+}
+
 _lib = None
 
 
@@ -186,7 +251,7 @@ def load():
     if not os.path.exists(path):
         raise RuntimeError("CUDA sampler library missing: %s (run python -m mantle_b200.build)" % path)
     L = C.CDLL(path)
-    for name, (res, args) in list(EXPORTS.items()) + list(HOST_EXPORTS.items()) + list(BATCH_EXPORTS.items()):
+    for name, (res, args) in [e for part in (EXPORTS, HOST_EXPORTS, BATCH_EXPORTS, HEAD_EXPORTS) for e in part.items()]:
         f = getattr(L, name)  # AttributeError here means the build is broken: do not hide it
         f.restype = res
         f.argtypes = args
