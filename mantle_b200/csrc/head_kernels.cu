@@ -114,8 +114,10 @@ const char* head_fault(const MantleHeadBatch* b) {
 
 // Everything about a batch that follows from its sizes: the tiling, what runs, and where in the workspace things lie.
 struct HeadLayout {
-    bool eight, adapters, sorted;  // sorted: x is read from the workspace's copy
-    int tile_cols, row_tiles, v_tiles, w_steps, chunks, slot_bound, box_bound;
+    bool eight, adapters;
+    bool sorted;  // rows in the order of their adapters
+    bool copied;  // x is read from the workspace's copy
+    int tile_cols, row_tiles, v_tiles, w_steps, u_cols, chunks, slot_bound, box_bound, u_rows;
     int stages, stage_bytes, grid;
     size_t smem;
     size_t perm, slots, boxes, tile_first, n_boxes, u, xs, total;
@@ -127,11 +129,10 @@ HeadLayout head_layout(const MantleHeadBatch* b) {
     l.eight = b->dtype == MANTLE_DTYPE_E4M3;
     l.adapters = b->n_adapters > 0;
     const bool aligned = on(b->hidden_rows, 16) && b->hidden_stride * (int64_t)e % 16 == 0;
-    l.sorted = l.adapters || !aligned;
     const bool weight = b->weight != nullptr;
-    // 8-bit operands with adapters need two accumulators, 128 columns each
-    const int max_cols = l.eight && l.adapters && weight ? MAX_COLS / 2 : MAX_COLS;
-    l.row_tiles = (b->rows + max_cols - 1) / max_cols;
+    l.sorted = l.adapters && b->rows > HERE_ROWS;
+    l.copied = weight && (l.sorted || !aligned);  // beside a projection x is only read by the shrink kernels
+    l.row_tiles = (b->rows + MAX_COLS - 1) / MAX_COLS;
     l.tile_cols = ((b->rows + l.row_tiles - 1) / l.row_tiles + WINDOW - 1) / WINDOW * WINDOW;
     l.row_tiles = (b->rows + l.tile_cols - 1) / l.tile_cols;
     l.v_tiles = (b->vocab + VT - 1) / VT;
@@ -139,9 +140,11 @@ HeadLayout head_layout(const MantleHeadBatch* b) {
     const int sms = device_info().sms;
     l.grid = l.row_tiles == 1 ? std::min(sms, (b->vocab + UNIT - 1) / UNIT)
                               : (int)std::min<long long>(sms, (long long)l.v_tiles * l.row_tiles);
-    const bool zero_first = l.adapters && (l.eight || !weight);
-    const size_t fixed = 1024 + sizeof(HeadCtl) + (zero_first ? ZERO_BYTES : 0);
-    l.stage_bytes = A_BYTES + l.tile_cols * STEP_BYTES;
+    const bool own_round = l.adapters && (l.eight || !weight);
+    const size_t fixed = 1024 + sizeof(HeadCtl) + (own_round ? ZERO_BYTES : 0);
+    // Adapters on the whole tile: room for four windows of u, as far as that is no more than W's share of the stage.
+    const int x_bytes = l.tile_cols * STEP_BYTES;
+    l.stage_bytes = A_BYTES + (l.adapters && !l.sorted ? std::max(x_bytes, std::min(2 * x_bytes, A_BYTES)) : x_bytes);
     l.stages = (int)std::min<size_t>(MAX_STAGES, ((size_t)232448 - fixed) / (size_t)l.stage_bytes);
     l.smem = fixed + (size_t)l.stages * (size_t)l.stage_bytes;
 
@@ -151,21 +154,25 @@ HeadLayout head_layout(const MantleHeadBatch* b) {
         return at;
     };
     if (l.adapters) {
-        l.chunks = (b->rank + U_CHUNK - 1) / U_CHUNK;
-        // a piece per adapter in use and one per cut; each box holds a row at least, and a piece of n rows touches
-        // at most n / 16 + 2 boxes
-        const int cuts = l.row_tiles * ((l.tile_cols + SLOT_COLS - 1) / SLOT_COLS);
-        l.slot_bound = std::min(b->rows, std::min(b->rows, b->n_adapters) + cuts);
-        l.box_bound = std::min(b->rows, b->rows / WINDOW + 2 * l.slot_bound);
-        l.perm = take((size_t)b->rows * 4);
+        l.u_cols = b->rank <= 16 ? 16 : 32;
+        l.chunks = (b->rank + l.u_cols - 1) / l.u_cols;
+        l.slot_bound = std::min(b->rows, b->n_adapters);
+        if (l.sorted) {
+            // a piece per adapter in use and one per cut; each box holds a row at least, and a piece of n rows touches
+            // at most n / 16 + 2 boxes
+            const int cuts = l.row_tiles * ((l.tile_cols + SLOT_COLS - 1) / SLOT_COLS);
+            l.slot_bound = std::min(b->rows, l.slot_bound + cuts);
+            l.box_bound = std::min(b->rows, b->rows / WINDOW + 2 * l.slot_bound);
+            l.perm = take((size_t)b->rows * 4);
+            l.boxes = take((size_t)l.box_bound * sizeof(HeadBox));
+            l.n_boxes = take(4);
+        }
+        l.u_rows = l.sorted ? l.box_bound * WINDOW : l.slot_bound * l.tile_cols;
         l.slots = take((size_t)l.slot_bound * sizeof(HeadSlot));
-        l.boxes = take((size_t)l.box_bound * sizeof(HeadBox));
         l.tile_first = take((size_t)(l.row_tiles + 1) * 4);
-        l.n_boxes = take(4);
-        l.u = take((size_t)l.chunks * (size_t)l.box_bound * WINDOW * U_ROW * 2);
+        l.u = take((size_t)l.chunks * (size_t)l.u_rows * (size_t)l.u_cols * 4);
     }
-    // beside a projection x is only read by the shrink kernel
-    if (l.sorted && weight) l.xs = take((size_t)b->rows * (size_t)b->hidden * e);
+    if (l.copied) l.xs = take((size_t)b->rows * (size_t)b->hidden * e);
     return l;
 }
 
@@ -202,11 +209,16 @@ bool encode_rows(CUtensorMap* m, const void* p, bool eight, long long rows, long
     const cuuint32_t box[2] = {(cuuint32_t)(STEP_BYTES / (eight ? 1 : 2)), (cuuint32_t)box_rows};
     return encode(m, p, eight, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
-bool encode_b(CUtensorMap* m, const MantleHeadBatch* b, int box_rows) {
+bool encode_u(CUtensorMap* m, const void* p, const HeadLayout& l, int box_rows) {
+    const cuuint64_t dims[2] = {(cuuint64_t)l.u_cols * 2, (cuuint64_t)l.chunks * (cuuint64_t)l.u_rows}, strides[1] = {(cuuint64_t)l.u_cols * 4};
+    const cuuint32_t box[2] = {(cuuint32_t)l.u_cols * 2, (cuuint32_t)box_rows};
+    return encode(m, p, false, 2, dims, strides, box, l.u_cols == 16 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B);
+}
+bool encode_b(CUtensorMap* m, const MantleHeadBatch* b, const HeadLayout& l, int box_rows) {
     const cuuint64_t dims[3] = {(cuuint64_t)b->rank, (cuuint64_t)b->vocab, (cuuint64_t)b->n_adapters};
     const cuuint64_t strides[2] = {(cuuint64_t)b->rank * 2, (cuuint64_t)b->rank * 2 * (cuuint64_t)b->vocab};
-    const cuuint32_t box[3] = {(cuuint32_t)U_CHUNK, (cuuint32_t)box_rows, 1};
-    return encode(m, b->adapter_b, false, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_64B);
+    const cuuint32_t box[3] = {(cuuint32_t)l.u_cols, (cuuint32_t)box_rows, 1};
+    return encode(m, b->adapter_b, false, 3, dims, strides, box, l.u_cols == 16 ? CU_TENSOR_MAP_SWIZZLE_32B : CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
 template <class... Args>
@@ -224,12 +236,21 @@ int launch(void (*kern)(Args...), dim3 grid, int threads, size_t smem, cudaStrea
     return (int)cudaLaunchKernelEx(&cfg, kern, args...);
 }
 
-template <bool E4M3>
-int launch_head(const HeadArgs& a, const HeadMaps& maps, const HeadLayout& l, cudaStream_t stream) {
+template <bool E4M3, bool OUT16, int GROUPS>
+int launch_head_as(const HeadArgs& a, const HeadMaps& maps, const HeadLayout& l, cudaStream_t stream) {
     static std::atomic<int> granted[kMaxDevices];
-    const int rc = ensure_smem(head_rows_kernel<E4M3>, l.smem, granted);
+    const auto kern = head_rows_kernel<E4M3, OUT16, GROUPS>;
+    const int rc = ensure_smem(kern, l.smem, granted);
     if (rc) return rc;
-    return launch<HeadArgs, HeadMaps>(head_rows_kernel<E4M3>, dim3((unsigned)l.grid), HEAD_NT, l.smem, stream, l.sorted, a, maps);
+    return launch<HeadArgs, HeadMaps>(kern, dim3((unsigned)l.grid), HEAD_NT, l.smem, stream, l.adapters || l.copied, a, maps);
+}
+
+template <bool E4M3, bool OUT16>
+int launch_head(const HeadArgs& a, const HeadMaps& maps, const HeadLayout& l, cudaStream_t stream) {
+    if (l.tile_cols <= 32) return launch_head_as<E4M3, OUT16, 1>(a, maps, l, stream);
+    if (l.tile_cols <= 64) return launch_head_as<E4M3, OUT16, 2>(a, maps, l, stream);
+    if (l.tile_cols <= 128) return launch_head_as<E4M3, OUT16, 4>(a, maps, l, stream);
+    return launch_head_as<E4M3, OUT16, 8>(a, maps, l, stream);
 }
 
 }  // namespace
@@ -276,7 +297,7 @@ extern "C" int mantleCudaHeadLaunches(const MantleHeadBatch* b, int* launches) {
     const char* fault = launches ? head_fault(b) : "head: no place for the count";
     if (fault) return refuse(fault);
     const HeadLayout l = head_layout(b);
-    *launches = 1 + (l.sorted ? 1 : 0) + (l.adapters ? 1 : 0);
+    *launches = 1 + (l.adapters || l.copied ? 1 : 0) + (l.sorted ? 1 : 0);
     return 0;
 }
 
@@ -299,9 +320,12 @@ extern "C" int mantleCudaHeadRows(const MantleHeadBatch* b, void* workspace, siz
     a.row_tiles = l.row_tiles;
     a.v_tiles = l.v_tiles;
     a.slots_on = l.adapters;
+    a.sorted = l.sorted;
+    a.copied = l.copied;
     a.rank = b->rank;
-    a.chunks = l.chunks;
-    a.u_chunk_rows = l.box_bound * WINDOW;
+    a.u_cols = l.u_cols;
+    a.u_rows = l.u_rows;
+    a.u_box = l.sorted ? WINDOW : l.tile_cols;
     a.stages = l.stages;
     a.stage_bytes = l.stage_bytes;
     a.x_scales = b->hidden_scales;
@@ -310,7 +334,6 @@ extern "C" int mantleCudaHeadRows(const MantleHeadBatch* b, void* workspace, siz
     a.out = b->out;
     a.base_stride = b->base_stride;
     a.out_stride = b->out_stride;
-    a.out_bf16 = b->out_dtype == MANTLE_DTYPE_BF16;
     a.status = b->status;
 
     HeadPrep p = {};
@@ -326,23 +349,26 @@ extern "C" int mantleCudaHeadRows(const MantleHeadBatch* b, void* workspace, siz
     p.vec = on(b->hidden_rows, 16) && b->hidden_stride * e % 16 == 0;
     p.n_adapters = b->n_adapters;
     p.rank = b->rank;
-    p.chunks = l.chunks;
+    p.u_cols = l.u_cols;
+    p.u_rows = l.u_rows;
     p.tile_cols = l.tile_cols;
     p.row_tiles = l.row_tiles;
-    p.box_bound = l.box_bound;
-    p.copy_ctas = l.sorted && b->weight ? std::min((b->rows + 7) / 8, 2 * device_info().sms) : 0;
+    p.units = l.sorted ? l.box_bound : l.slot_bound;
+    p.copy_ctas = l.copied ? std::min((b->rows + SHRINK_WARPS - 1) / SHRINK_WARPS, 2 * device_info().sms) : 0;
     if (l.adapters) {
-        p.perm = reinterpret_cast<int*>(ws + l.perm);
         p.slots = reinterpret_cast<HeadSlot*>(ws + l.slots);
-        p.boxes = reinterpret_cast<HeadBox*>(ws + l.boxes);
         p.tile_first = reinterpret_cast<int*>(ws + l.tile_first);
-        p.n_boxes = reinterpret_cast<int*>(ws + l.n_boxes);
         p.u = reinterpret_cast<bf16_raw*>(ws + l.u);
-        a.perm = p.perm;
         a.slots = p.slots;
         a.tile_first = p.tile_first;
     }
-    if (p.copy_ctas) p.xs = ws + l.xs;
+    if (l.sorted) {
+        p.perm = reinterpret_cast<int*>(ws + l.perm);
+        p.boxes = reinterpret_cast<HeadBox*>(ws + l.boxes);
+        p.n_boxes = reinterpret_cast<int*>(ws + l.n_boxes);
+        a.perm = p.perm;
+    }
+    if (l.copied) p.xs = ws + l.xs;
 
     HeadMaps maps;
     memset(&maps, 0, sizeof maps);
@@ -354,21 +380,23 @@ extern "C" int mantleCudaHeadRows(const MantleHeadBatch* b, void* workspace, siz
                          : encode_rows(&maps.x, b->hidden_rows, l.eight, b->rows, b->hidden, b->hidden_stride * e, l.tile_cols));
     }
     if (l.adapters) {
-        ok = ok && encode_b(&maps.b, b, VT) && encode_b(&maps.b16, b, UNIT);
-        const long long u_rows = (long long)l.chunks * l.box_bound * WINDOW;
-        ok = ok && encode_rows(&maps.u, p.u, false, u_rows, U_ROW, U_ROW * 2, WINDOW);
+        ok = ok && encode_b(&maps.b, b, l, VT) && encode_b(&maps.b16, b, l, UNIT);
+        ok = ok && encode_u(&maps.u, p.u, l, a.u_box);
     }
     if (!ok) return refuse("head: the driver refused a tensor map");
 
     int rc = 0;
-    if (l.adapters) {
+    if (l.sorted) {
         rc = launch<HeadPrep>(head_sort_kernel, dim3(1), SORT_NT, ((size_t)b->n_adapters + 1) * 4, stream, false, p);
         if (rc) return rc;
     }
-    if (l.sorted) {
-        const dim3 grid((unsigned)(l.box_bound + p.copy_ctas), (unsigned)std::max(1, l.adapters ? b->rank / 8 : 1));
-        rc = launch<HeadPrep>(head_shrink_kernel, grid, 256, 0, stream, l.adapters, p);
+    if (l.adapters || l.copied) {
+        const dim3 grid((unsigned)(p.units + p.copy_ctas), (unsigned)(l.adapters ? b->rank / 8 : 1));
+        rc = l.sorted ? launch<HeadPrep>(head_shrink_kernel, grid, SHRINK_NT, 0, stream, true, p)
+                      : launch<HeadPrep>(head_shrink_here_kernel, grid, SHRINK_NT, 0, stream, false, p);
         if (rc) return rc;
     }
-    return l.eight ? launch_head<true>(a, maps, l, stream) : launch_head<false>(a, maps, l, stream);
+    if (b->out_dtype == MANTLE_DTYPE_BF16)
+        return l.eight ? launch_head<true, true>(a, maps, l, stream) : launch_head<false, true>(a, maps, l, stream);
+    return l.eight ? launch_head<true, false>(a, maps, l, stream) : launch_head<false, false>(a, maps, l, stream);
 }

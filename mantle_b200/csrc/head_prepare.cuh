@@ -6,28 +6,34 @@
 //
 //     D[v][row] += sum_j B[a][v][j] * u[row][j],     u[row][j] = gain[a] * sum_k x^[row][k] A[a][j][k]
 //
-// for the rows that use adapter a.  For that the rows are put in an order in which those of one adapter
-// stand together (head_sort_kernel), so that such a step covers a window of neighbouring columns of D and
-// not the whole tile; u is laid out per window with zeros for the columns that belong to other rows
-// (head_shrink_kernel), which makes the windows' products plain sums.  A row's result does not depend on
-// where in the order it stands: a column of D only ever sees its own column of the operands.
+// on a window of neighbouring columns of D, with zeros in u for the columns there that belong to rows of other
+// adapters; a slot is one such step.  A row's result depends neither on where it stands in the tile nor on what
+// stands beside it: a column of D only ever sees its own column of the operands, and adding zeros to it changes
+// nothing.
+//
+// Two forms.  Up to HERE_ROWS rows, one kernel: rows stay where they are, and an adapter's window is the whole
+// tile, zeros and all; the projection can then read x and W from its first cycle on, and meets this kernel's
+// results only when it comes to the adapters.  More rows: head_sort_kernel puts the rows in an order in which
+// those of one adapter stand together, and head_shrink_kernel copies x in that order, so that a window covers an
+// adapter's own rows and little else.
 #pragma once
 
 namespace {
 
-constexpr int U_CHUNK = 32;        // ranks of one step: a row of u holds 32 leading parts and 32 remainders
-constexpr int U_ROW = 2 * U_CHUNK; // bfloat16 elements, 128 bytes
 constexpr int WINDOW = 16;         // columns of D come in sixteens
-constexpr int SLOT_COLS = 128;     // a slot's window lies within an aligned run of 128 columns of its tile
+constexpr int SLOT_COLS = 128;     // sorted: a slot's window lies within an aligned run of 128 columns of its tile
+constexpr int HERE_ROWS = 128;
 constexpr int SORT_NT = 1024;
+constexpr int SHRINK_NT = 512;
+constexpr int SHRINK_WARPS = SHRINK_NT / 32;
 
 // One step's worth of columns: adapter `adapter` on columns [col, col + n) of its row tile, with the rows of u
 // from u_row on.  16 bytes, read as one int4.
-struct HeadSlot {
+struct __align__(16) HeadSlot {
     int adapter, col, n, u_row;
 };
 // Sixteen rows of u: sorted places [place, place + 16), of which [first, last) use the adapter.
-struct HeadBox {
+struct __align__(16) HeadBox {
     int adapter, place, first, last;
 };
 
@@ -40,17 +46,19 @@ struct HeadPrep {
     const int32_t* ids;
     long long x_stride;  // elements
     int rows, hidden, e4m3, vec;  // vec: rows of x start on 16 bytes
-    int n_adapters, rank, chunks;
+    int n_adapters, rank;
+    int u_cols;          // ranks of one step, 16 or 32: a row of u holds as many leading parts, then as many remainders
+    int u_rows;          // rows of u of one chunk of ranks
     int tile_cols, row_tiles;
-    int box_bound, copy_ctas;
+    int units, copy_ctas;  // CTAs of the shrink kernel: slots or boxes at most; and those that copy x
     // workspace
     int* perm;        // [rows] sorted place -> row
     HeadSlot* slots;
     HeadBox* boxes;
     int* tile_first;  // [row_tiles + 1] first slot of a tile
     int* n_boxes;     // [1]
-    bf16_raw* u;      // [chunks][16 * box_bound][U_ROW]
-    void* xs;         // [rows][hidden] sorted, contiguous
+    bf16_raw* u;      // [chunks][u_rows][2 * u_cols]
+    void* xs;         // [rows][hidden] contiguous, sorted
 };
 
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
@@ -192,51 +200,44 @@ __device__ __forceinline__ uint4 x_eight(const HeadPrep& p, const char* row, int
                       q[6] | (uint32_t)q[7] << 16);
 }
 
-// CTAs [0, box_bound) x [0, rank / 8): eight ranks of sixteen rows of u.  The warps share out the columns of x
-// and add their sums up in shared memory.  The order of the columns within a step is free in a dot product, so
-// each lane takes eight neighbours of its row, one 16-byte load, as two steps' operands.
-// CTAs from box_bound on (blockIdx.y 0): the sorted copy of x.
-__global__ void __launch_bounds__(256) head_shrink_kernel(const HeadPrep p) {
-    __shared__ float sums[8][16][8];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int esz = p.e4m3 ? 1 : 2;
-    pdl_trigger();
-    pdl_wait();
-    if ((int)blockIdx.x >= p.box_bound) {
-        if (blockIdx.y) return;
-        const int w0 = ((int)blockIdx.x - p.box_bound) * 8 + warp;
-        const long long bytes = (long long)p.hidden * esz;  // a multiple of 16
-        for (int r = w0; r < p.rows; r += p.copy_ctas * 8) {
-            const int from = p.n_adapters ? p.perm[r] : r;
-            const char* src = static_cast<const char*>(p.x) + (long long)from * p.x_stride * esz;
-            char* dst = static_cast<char*>(p.xs) + r * bytes;
-            if (p.vec) {
-                for (long long i = lane * 16; i < bytes; i += 512) *reinterpret_cast<uint4*>(dst + i) = *reinterpret_cast<const uint4*>(src + i);
-            } else if (p.e4m3) {
-                for (long long i = lane; i < bytes; i += 32) dst[i] = src[i];
-            } else {
-                for (long long i = lane * 2; i < bytes; i += 64) *reinterpret_cast<bf16_raw*>(dst + i) = *reinterpret_cast<const bf16_raw*>(src + i);
-            }
+// The copy of x, in sorted order where there is one: one warp a row.
+__device__ __forceinline__ void copy_rows(const HeadPrep& p, int first, int step) {
+    const int lane = threadIdx.x & 31, esz = p.e4m3 ? 1 : 2;
+    const long long bytes = (long long)p.hidden * esz;  // a multiple of 16
+    for (int r = first; r < p.rows; r += step) {
+        const int from = p.perm ? p.perm[r] : r;
+        const char* src = static_cast<const char*>(p.x) + (long long)from * p.x_stride * esz;
+        char* dst = static_cast<char*>(p.xs) + r * bytes;
+        if (p.vec) {
+            for (long long i = lane * 16; i < bytes; i += 512)
+                *reinterpret_cast<uint4*>(dst + i) = *reinterpret_cast<const uint4*>(src + i);
+        } else if (p.e4m3) {
+            for (long long i = lane; i < bytes; i += 32) dst[i] = src[i];
+        } else {
+            for (long long i = lane * 2; i < bytes; i += 64)
+                *reinterpret_cast<bf16_raw*>(dst + i) = *reinterpret_cast<const bf16_raw*>(src + i);
         }
-        return;
     }
-    if ((int)blockIdx.x >= *p.n_boxes) return;
-    const HeadBox box = p.boxes[blockIdx.x];
-    const int adapter = box.adapter, place = box.place, first = box.first, last = box.last;
-    const int j0 = blockIdx.y * 8;
-    const int g = lane >> 2, q = lane & 3;
-    // the two rows of x this lane loads from (null: zeros), and its row of A
+}
+
+// Eight ranks (from j0) of sixteen rows' products with one adapter's A: rows[i] is the row of x of place i, -1 none.
+// The warps share out the columns of x and add their sums up in shared memory.  The order of the columns within
+// a step is free in a dot product, so each lane takes eight neighbours of its row, one 16-byte load, as two
+// steps' operands.  On return thread i * 8 + j of the first 128 holds place i, rank j0 + j.
+__device__ __forceinline__ float shrink16(const HeadPrep& p, int adapter, int j0, const int* rows, float (*sums)[16][8]) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+    const int esz = p.e4m3 ? 1 : 2;
     const char* row[2];
 #pragma unroll
     for (int i = 0; i < 2; i++) {
-        const int at = place + g + 8 * i;
-        row[i] = at >= first && at < last ? static_cast<const char*>(p.x) + (long long)p.perm[at] * p.x_stride * esz : nullptr;
+        const int r = rows[g + 8 * i];
+        row[i] = r >= 0 ? static_cast<const char*>(p.x) + (long long)r * p.x_stride * esz : nullptr;
     }
     const bf16_raw* arow = p.a + ((long long)adapter * p.rank + j0 + g) * p.hidden;
     float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     const uint4 none = make_uint4(0, 0, 0, 0);
 #pragma unroll 4
-    for (int k = warp * 32 + q * 8; k < p.hidden + q * 8; k += 256) {  // the same count for a warp's lanes
+    for (int k = warp * 32 + q * 8; k < p.hidden + q * 8; k += SHRINK_WARPS * 32) {  // the same count for a warp's lanes
         const bool in = k < p.hidden;
         const uint4 b = in ? *reinterpret_cast<const uint4*>(arow + k) : none;
         const uint4 x0 = in && row[0] ? x_eight(p, row[0], k) : none;
@@ -247,27 +248,125 @@ __global__ void __launch_bounds__(256) head_shrink_kernel(const HeadPrep p) {
     sums[warp][g][q * 2] = d[0], sums[warp][g][q * 2 + 1] = d[1];
     sums[warp][g + 8][q * 2] = d[2], sums[warp][g + 8][q * 2 + 1] = d[3];
     __syncthreads();
-    if (threadIdx.x >= 128) return;
-    const int i = threadIdx.x >> 3, j = threadIdx.x & 7, at = place + i;
     float v = 0.0f;
-    if (at >= first && at < last) {
+    if (threadIdx.x < 128) {
+        const int i = threadIdx.x >> 3, j = threadIdx.x & 7, r = rows[i];
+        if (r >= 0) {
 #pragma unroll
-        for (int w = 0; w < 8; w++) v += sums[w][i][j];
-        if (p.gain) v *= p.gain[adapter];
-        if (p.e4m3) v *= p.x_scales[p.perm[at]];
+            for (int w = 0; w < SHRINK_WARPS; w++) v += sums[w][i][j];
+            if (p.gain) v *= p.gain[adapter];
+            if (p.e4m3) v *= p.x_scales[r];
+        }
     }
-    // v in two bfloat16: 16 bits of mantissa (an infinity or NaN stays in the leading part alone)
+    return v;
+}
+
+// v in two bfloat16: 16 bits of mantissa (an infinity or NaN stays in the leading part alone).  Where the rank ends
+// inside a step of sixteen, the thread of its last eight also writes the zeros behind them.
+__device__ __forceinline__ void store_u(const HeadPrep& p, int rank_at, int u_row, float v) {
     const uint32_t hi = pack_bf16(v, 0.0f) & 0xffffu;
     const float rest = v - __uint_as_float(hi << 16);
     const uint32_t lo = (hi & 0x7f80u) == 0x7f80u ? 0u : pack_bf16(rest, 0.0f) & 0xffffu;
-    const int rank_at = j0 + j, chunk = rank_at / U_CHUNK;
-    bf16_raw* u = p.u + (((long long)chunk * p.box_bound + blockIdx.x) * WINDOW + i) * U_ROW + rank_at % U_CHUNK;
+    bf16_raw* u = p.u + ((long long)(rank_at / p.u_cols) * p.u_rows + u_row) * (2 * p.u_cols) + rank_at % p.u_cols;
     u[0] = (bf16_raw)hi;
-    u[U_CHUNK] = (bf16_raw)lo;
-    // a rank that ends inside a step of sixteen: zeros up to its end
+    u[p.u_cols] = (bf16_raw)lo;
     if (rank_at + 8 >= p.rank && p.rank % 16) {
         u[8] = 0;
-        u[U_CHUNK + 8] = 0;
+        u[p.u_cols + 8] = 0;
+    }
+}
+
+// Sorted form.  CTAs [0, units) x [0, rank / 8): eight ranks of one box.  CTAs from `units` on: the copy of x.
+__global__ void __launch_bounds__(SHRINK_NT) head_shrink_kernel(const HeadPrep p) {
+    __shared__ float sums[SHRINK_WARPS][16][8];
+    __shared__ int rows[16];
+    pdl_trigger();
+    pdl_wait();
+    if ((int)blockIdx.x >= p.units) {
+        if (blockIdx.y == 0)
+            copy_rows(p, ((int)blockIdx.x - p.units) * SHRINK_WARPS + (int)(threadIdx.x >> 5), p.copy_ctas * SHRINK_WARPS);
+        return;
+    }
+    if ((int)blockIdx.x >= *p.n_boxes) return;
+    const HeadBox box = p.boxes[blockIdx.x];
+    if (threadIdx.x < 16) {
+        const int at = box.place + (int)threadIdx.x;
+        rows[threadIdx.x] = at >= box.first && at < box.last ? p.perm[at] : -1;
+    }
+    __syncthreads();
+    const int j0 = blockIdx.y * 8;
+    const float v = shrink16(p, box.adapter, j0, rows, sums);
+    if (threadIdx.x < 128) store_u(p, j0 + (int)(threadIdx.x & 7), (int)blockIdx.x * WINDOW + (int)(threadIdx.x >> 3), v);
+}
+
+// Form for up to HERE_ROWS rows.  CTAs [0, units) x [0, rank / 8): eight ranks of the rows of one adapter -- the
+// blockIdx.x-th of those in use, in the order of their first rows -- and zeros for the others.  CTAs from `units` on:
+// the copy of x, where its rows do not start on 16 bytes.
+__global__ void __launch_bounds__(SHRINK_NT) head_shrink_here_kernel(const HeadPrep p) {
+    __shared__ float sums[SHRINK_WARPS][16][8];
+    __shared__ __align__(16) int ids[HERE_ROWS];
+    __shared__ int mine[HERE_ROWS + 16], first_of[HERE_ROWS];
+    __shared__ int counts[2 * (HERE_ROWS / 32)];
+    pdl_trigger();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if ((int)blockIdx.x >= p.units) {
+        if (blockIdx.y == 0)
+            copy_rows(p, ((int)blockIdx.x - p.units) * SHRINK_WARPS + warp, p.copy_ctas * SHRINK_WARPS);
+        return;
+    }
+    // the adapters in use: a row is its adapter's first if no row before it has the same
+    if (tid < HERE_ROWS) {
+        const int id = tid < p.rows ? p.ids[tid] : -1;
+        ids[tid] = id >= 0 && id < p.n_adapters ? id : -1;
+        mine[tid] = -1;
+    }
+    if (tid < 16) mine[HERE_ROWS + tid] = -1;
+    __syncthreads();
+    if (tid < HERE_ROWS) {
+        const int id = ids[tid];
+        bool first = id >= 0;
+#pragma unroll 8
+        for (int r = 0; r < HERE_ROWS; r += 4) {
+            const int4 v = *reinterpret_cast<const int4*>(ids + r);
+            first = first && !(r < tid && v.x == id) && !(r + 1 < tid && v.y == id) && !(r + 2 < tid && v.z == id) && !(r + 3 < tid && v.w == id);
+        }
+        const uint32_t votes = __ballot_sync(0xffffffffu, first);
+        if (lane == 0) counts[warp] = __popc(votes);
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        int at = __popc(votes & ((1u << lane) - 1));
+        for (int w = 0; w < warp; w++) at += counts[w];
+        if (first) first_of[at] = tid;
+    }
+    __syncthreads();
+    int in_use = 0;
+    for (int w = 0; w < HERE_ROWS / 32; w++) in_use += counts[w];
+    if (blockIdx.x == 0 && blockIdx.y == 0) {
+        if (tid < in_use) {
+            HeadSlot s = {ids[first_of[tid]], 0, p.tile_cols, tid * p.tile_cols};
+            p.slots[tid] = s;
+        }
+        if (tid < 2) p.tile_first[tid] = tid ? in_use : 0;
+    }
+    if ((int)blockIdx.x >= in_use) return;
+    const int adapter = ids[first_of[blockIdx.x]], j0 = blockIdx.y * 8, u_row = (int)blockIdx.x * p.tile_cols;
+    if (tid < HERE_ROWS) {
+        const bool use = ids[tid] == adapter;
+        const uint32_t votes = __ballot_sync(0xffffffffu, use);
+        if (lane == 0) counts[HERE_ROWS / 32 + warp] = __popc(votes);
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        int at = __popc(votes & ((1u << lane) - 1));
+        for (int w = 0; w < warp; w++) at += counts[HERE_ROWS / 32 + w];
+        if (use) mine[at] = tid;
+    }
+    for (int i = tid; i < p.tile_cols * 8; i += SHRINK_NT)
+        if (i / 8 >= HERE_ROWS || ids[i / 8] != adapter) store_u(p, j0 + i % 8, u_row + i / 8, 0.0f);
+    __syncthreads();
+    int n = 0;
+    for (int w = 0; w < HERE_ROWS / 32; w++) n += counts[HERE_ROWS / 32 + w];
+    for (int i = 0; i < n; i += 16) {
+        const float v = shrink16(p, adapter, j0, mine + i, sums);
+        if (tid < 128 && i + (tid >> 3) < n) store_u(p, j0 + (tid & 7), u_row + mine[i + (tid >> 3)], v);
+        __syncthreads();
     }
 }
 

@@ -8,16 +8,20 @@
 // writes 32 neighbouring columns of a row of logits per warp.  W and B pass through the SM once per tile of
 // rows, whatever the number of rows.
 //
-// One CTA per SM, persistent over its tiles.  Warp 4 moves operands with TMA into a ring of stages (a stage: 128
-// rows of W, 128 bytes wide, and the same slice of x; or 32 ranks of one adapter's B and its window of u), warp 5
-// issues tcgen05.mma from it, warps 0-3 read finished accumulators out of tensor memory and write them while
-// the next tile is computed into the other half.
+// One CTA per SM, persistent over its tiles.  Warp 8 moves operands with TMA into a ring of stages (a stage: 128
+// rows of W, 128 bytes wide, and the same slice of x; or some adapters' B, 16 or 32 ranks wide, and their windows of
+// u), warp 9 issues tcgen05.mma from it, warps 0-7 read accumulators out of tensor memory, add them up in
+// registers and write the finished tile while the next one is computed.
 //
-// u comes as two bfloat16, leading part and remainder, side by side in a row of 128 bytes: two products with
-// the same B, which cost no more bytes, keep 16 bits of it.
+// Rounds.  A float32 accumulator in tensor memory is cut, not rounded, at every step, so its error grows with the
+// number of steps, always towards zero (measured with bfloat16 operands: 2.3e-7 of the result after 256 columns,
+// 9.1e-6 after 8192).  A tile is therefore computed in rounds of 512 columns, each in a fresh one of two
+// accumulators, and the rounds are added with ordinary float32 sums (5e-7 at any width).  With e4m3 operands the
+// products are short and the cut costs nothing that shows (5.1e-7 after 8192 columns): a round is 8192 columns.
 //
-// With 8-bit operands the projection's accumulator has to be scaled by row and column before the adapters'
-// part is added, so the two have accumulators of their own (128 rows a tile at most).
+// u comes as two bfloat16, leading part and remainder, side by side: two products with the same B, which cost no more
+// bytes, keep 16 bits of it.  With 8-bit operands the projection's rounds are scaled by row and column, and the
+// adapters have a round of their own.
 #pragma once
 
 namespace {
@@ -28,20 +32,25 @@ constexpr int A_BYTES = VT * STEP_BYTES;
 constexpr int MAX_COLS = 256;
 constexpr int MAX_STAGES = 12;
 constexpr int UNIT = 16;           // vocabulary rows by which single-tile batches are shared out
-constexpr int HEAD_NT = 192;
+constexpr int ROUND_BF16 = 8;      // steps of a round
+constexpr int ROUND_E4M3 = 64;
+constexpr int WRITERS = 256;       // threads that read accumulators and write results
+constexpr int HEAD_NT = WRITERS + 64;
 constexpr int ZERO_BYTES = MAX_COLS * 32;
+constexpr int MAX_PACK = 4;        // adapters' steps in one stage
 
 struct HeadCtl {
     uint64_t full[MAX_STAGES], empty[MAX_STAGES], acc_full[2], acc_empty[2], drain;
     uint32_t tmem;
     int abort;
-    int row_of[MAX_COLS];
+    long long out_of[MAX_COLS], base_of[MAX_COLS];  // a column's row, as a distance in bytes
     float scale_of[MAX_COLS];
 };
 
 struct HeadArgs {
     int rows, vocab, w_steps, tile_cols, row_tiles, v_tiles;
-    int slots_on, rank, chunks, u_chunk_rows;
+    int slots_on, sorted, copied;  // adapters; perm and x come from the kernel in front
+    int rank, u_cols, u_rows, u_box;  // u_box: rows of u of one copy
     int stages, stage_bytes;
     const int* perm;
     const HeadSlot* slots;
@@ -51,7 +60,6 @@ struct HeadArgs {
     const void* base;
     void* out;
     long long base_stride, out_stride;
-    int out_bf16;
     int* status;
 };
 
@@ -78,12 +86,11 @@ __device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* map, int
 
 // Shared-memory matrix descriptor of a K-major operand: rows of 128, 64 or 32 bytes, swizzled by the same
 // width, eight rows to a group and the groups one after the other.
-enum : uint64_t { SWIZZLE_128 = 2, SWIZZLE_64 = 4, SWIZZLE_32 = 6 };
-template <uint64_t SWIZZLE>
-__device__ __forceinline__ uint64_t operand(uint32_t addr) {
-    constexpr uint64_t row = SWIZZLE == SWIZZLE_128 ? 128 : SWIZZLE == SWIZZLE_64 ? 64 : 32;
-    return (uint64_t)((addr >> 4) & 0x3fff) | (uint64_t)1 << 16 | (row * 8 >> 4) << 32 | (uint64_t)1 << 46 | SWIZZLE << 61;
+__device__ __forceinline__ uint64_t operand_format(int row_bytes) {
+    const uint64_t swizzle = row_bytes == 128 ? 2 : row_bytes == 64 ? 4 : 6;
+    return (uint64_t)1 << 16 | (uint64_t)(row_bytes * 8 >> 4) << 32 | (uint64_t)1 << 46 | swizzle << 61;
 }
+__device__ __forceinline__ uint64_t operand(uint64_t format, uint32_t addr) { return format | (uint64_t)((addr >> 4) & 0x3fff); }
 // Instruction descriptor: float32 accumulator, 128 x n; bfloat16 operands, or e4m3.
 __device__ __forceinline__ uint32_t shape_bf16(int n) {
     return 1u << 4 | 1u << 7 | 1u << 10 | (uint32_t)(n >> 3) << 17 | (uint32_t)(VT >> 4) << 24;
@@ -134,18 +141,19 @@ __device__ __forceinline__ bool head_wait(uint64_t* bar, uint32_t parity, volati
     }
 }
 
-// A barrier of the 128 threads that write results, and whether all of them are still in order.
-__device__ __forceinline__ bool epilogue_agree(bool ok) {
+// A barrier of the threads that write results, and whether all of them are still in order.
+__device__ __forceinline__ bool writers_agree(bool ok) {
     int all;
-    asm volatile("{.reg .pred p, q; setp.ne.b32 p, %1, 0; bar.red.and.pred q, 1, 128, p; selp.b32 %0, 1, 0, q;}"
+    asm volatile("{.reg .pred p, q; setp.ne.b32 p, %1, 0; bar.red.and.pred q, 1, 256, p; selp.b32 %0, 1, 0, q;}"
                  : "=r"(all) : "r"((int)ok) : "memory");
     return all != 0;
 }
 
 // The tiles of this CTA, one after the other.  One tile of rows: the vocabulary is shared out in equal runs of
 // 16-row units, so that every SM streams the same bytes (151 936 columns are 1187 tiles of 128: eight for each of
-// 148 SMs, and three left over); a run's last tile may be short.  Several tiles of rows: whole tiles, those of the
-// same vocabulary rows next to each other, so that W comes from HBM once and from L2 after that.
+// 148 SMs, and three left over); a run's short tile comes first, where the ring is filling anyway.  Several tiles of
+// rows: whole tiles, those of the same vocabulary rows next to each other, so that W comes from HBM once and from
+// L2 after that.
 struct HeadTiles {
     int unit, unit_end, t, n_tiles, row_tiles;
     __device__ explicit HeadTiles(const HeadArgs& a) {
@@ -160,10 +168,11 @@ struct HeadTiles {
     __device__ bool next(int* v0, int* v_rows, int* row_tile) {
         if (row_tiles == 1) {
             if (unit >= unit_end) return false;
+            const int odd = (unit_end - unit) % (VT / UNIT), n = odd ? odd : VT / UNIT;
             *v0 = unit * UNIT;
-            *v_rows = min(VT / UNIT, unit_end - unit) * UNIT;
+            *v_rows = n * UNIT;
             *row_tile = 0;
-            unit += VT / UNIT;
+            unit += n;
             return true;
         }
         if (t >= n_tiles) return false;
@@ -175,22 +184,70 @@ struct HeadTiles {
     }
 };
 
+// The adapters' steps of a tile, packed into stages as they come: up to the stage's room for B and for u.
+struct HeadPacks {
+    const HeadSlot* slots;
+    int at, end, chunk, chunks, most, room, row_bytes;
+    __device__ HeadPacks(const HeadArgs& a, int row_tile) {
+        slots = a.slots;
+        at = a.tile_first[row_tile];
+        end = a.tile_first[row_tile + 1];
+        chunk = 0;
+        chunks = (a.rank + a.u_cols - 1) / a.u_cols;
+        row_bytes = a.u_cols * 4;
+        most = A_BYTES / (VT * a.u_cols * 2);
+        room = a.stage_bytes - A_BYTES;
+    }
+    // The steps of the next stage; 0: no more.
+    __device__ int next(HeadSlot slot[MAX_PACK], int chunk_of[MAX_PACK], int* u_bytes) {
+        int n = 0;
+        *u_bytes = 0;
+#pragma unroll
+        for (int i = 0; i < MAX_PACK; i++) {
+            if (i < most && n == i && at < end) {
+                const HeadSlot s = slots[at];
+                if (*u_bytes + s.n * row_bytes <= room) {
+                    slot[i] = s;
+                    chunk_of[i] = chunk;
+                    *u_bytes += s.n * row_bytes;
+                    n++;
+                    if (++chunk == chunks) chunk = 0, at++;
+                }
+            }
+        }
+        return n;
+    }
+};
+
 // ---- the kernel
 
-template <bool E4M3>
+template <bool OUT16>
+struct OutType {
+    typedef float type;
+};
+template <>
+struct OutType<true> {
+    typedef bf16_raw type;
+};
+
+// GROUPS: a tile has up to 32 * GROUPS columns.  (The writers' part is unrolled over them, its sums being registers;
+// unrolled to 256 columns for every batch, a single row spent its time on fetching instructions: 88 against 58 us.)
+template <bool E4M3, bool OUT16, int GROUPS>
 __global__ void __launch_bounds__(HEAD_NT, 1) head_rows_kernel(const HeadArgs a, const __grid_constant__ HeadMaps maps) {
     extern __shared__ char raw[];
+    constexpr int STEP_COLS = E4M3 ? STEP_BYTES : STEP_BYTES / 2;
+    constexpr int ROUND = E4M3 ? ROUND_E4M3 : ROUND_BF16;
+    constexpr int OUT_BYTES = OUT16 ? 2 : 4;
+    using Out = typename OutType<OUT16>::type;
     const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
     char* const ring = raw + (base - smem_u32(raw));
     const uint32_t zeros = base + (uint32_t)(a.stages * a.stage_bytes);
-    const bool zero_first = a.slots_on && (E4M3 || a.w_steps == 0);
-    HeadCtl& ctl = *reinterpret_cast<HeadCtl*>(ring + a.stages * a.stage_bytes + (zero_first ? ZERO_BYTES : 0));
+    // the adapters have a round of their own, or are the end of the projection's last one
+    const bool own_round = a.slots_on && (E4M3 || a.w_steps == 0);
+    HeadCtl& ctl = *reinterpret_cast<HeadCtl*>(ring + a.stages * a.stage_bytes + (own_round ? ZERO_BYTES : 0));
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    // columns of tensor memory: two accumulators of 256, the adapters' part in the second 128 of each with e4m3
-    const uint32_t acc_of[2] = {0u, 256u};
-    const uint32_t slot_acc = E4M3 && a.w_steps ? 128u : 0u;
 
-    if (zero_first) {
+    if (own_round) {
         for (int i = threadIdx.x; i < ZERO_BYTES / 16; i += HEAD_NT)
             reinterpret_cast<uint4*>(ring + a.stages * a.stage_bytes)[i] = make_uint4(0, 0, 0, 0);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -202,13 +259,13 @@ __global__ void __launch_bounds__(HEAD_NT, 1) head_rows_kernel(const HeadArgs a,
         }
         for (int i = 0; i < 2; i++) {
             mbar_init(&ctl.acc_full[i], 1);
-            mbar_init(&ctl.acc_empty[i], 4);
+            mbar_init(&ctl.acc_empty[i], WRITERS / 32);
         }
         mbar_init(&ctl.drain, 1);
         ctl.abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 5) {
+    if (warp == WRITERS / 32 + 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&ctl.tmem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
         tmem_fence_before();
@@ -218,13 +275,19 @@ __global__ void __launch_bounds__(HEAD_NT, 1) head_rows_kernel(const HeadArgs a,
     const uint32_t tmem = ctl.tmem;
     HeadTiles tiles(a);
     int v0, v_rows, row_tile;
+    // what the kernels in front wrote may be read from here on (each thread asks once, where it first needs it)
+    bool behind = false;
+    auto wait_for_front = [&]() {
+        if (!behind) pdl_wait();
+        behind = true;
+    };
 
-    if (warp == 4) {
+    if (warp == WRITERS / 32) {
         if (lane == 0) {
             // fills of the ring, counted from the start; stage fill % stages
             int fill = 0, stage = 0;
             uint32_t phase = 1;  // of `empty`: the first round passes
-            bool ok = true, waited = false;
+            bool ok = true;
             auto take = [&]() { ok = head_wait(&ctl.empty[stage], phase, &ctl.abort); return ok; };
             auto advance = [&]() {
                 fill++;
@@ -233,30 +296,27 @@ __global__ void __launch_bounds__(HEAD_NT, 1) head_rows_kernel(const HeadArgs a,
             auto load_w = [&](int s) {
                 const uint32_t dst = base + (uint32_t)(stage * a.stage_bytes);
                 mbar_expect(&ctl.full[stage], (uint32_t)((v_rows + a.tile_cols) * STEP_BYTES));
-                const int x = s * (E4M3 ? STEP_BYTES : STEP_BYTES / 2);
                 if (v_rows == VT) {
-                    tma_2d(dst, &maps.w, x, v0, &ctl.full[stage]);
+                    tma_2d(dst, &maps.w, s * STEP_COLS, v0, &ctl.full[stage]);
                 } else {
-                    for (int i = 0; i < v_rows; i += UNIT) tma_2d(dst + i * STEP_BYTES, &maps.w16, x, v0 + i, &ctl.full[stage]);
+                    for (int i = 0; i < v_rows; i += UNIT) tma_2d(dst + i * STEP_BYTES, &maps.w16, s * STEP_COLS, v0 + i, &ctl.full[stage]);
                 }
             };
             auto load_x = [&](int s, int st) {
-                tma_2d(base + (uint32_t)(st * a.stage_bytes + A_BYTES), &maps.x, s * (E4M3 ? STEP_BYTES : STEP_BYTES / 2),
-                       row_tile * a.tile_cols, &ctl.full[st]);
+                tma_2d(base + (uint32_t)(st * a.stage_bytes + A_BYTES), &maps.x, s * STEP_COLS, row_tile * a.tile_cols, &ctl.full[st]);
             };
             while (ok && tiles.next(&v0, &v_rows, &row_tile)) {
                 int s = 0;
-                if (!waited) {
+                if (a.copied && !behind) {
                     // W does not come from the kernels in front: the ring fills with it while they still run
                     const int ahead = min(a.stages, a.w_steps);
                     for (; s < ahead; s++) {
                         load_w(s);
                         advance();
                     }
-                    pdl_wait();
+                    wait_for_front();
                     asm volatile("fence.proxy.async.global;" ::: "memory");
                     for (int i = 0; i < ahead; i++) load_x(i, i);
-                    waited = true;
                 }
                 for (; s < a.w_steps; s++) {
                     if (!take()) break;
@@ -265,24 +325,34 @@ __global__ void __launch_bounds__(HEAD_NT, 1) head_rows_kernel(const HeadArgs a,
                     advance();
                 }
                 if (!ok || !a.slots_on) continue;
-                const int end = a.tile_first[row_tile + 1];
-                for (int i = a.tile_first[row_tile]; i < end && ok; i++) {
-                    const HeadSlot slot = a.slots[i];
-                    for (int c = 0; c < a.chunks; c++) {
-                        if (!take()) break;
-                        const uint32_t dst = base + (uint32_t)(stage * a.stage_bytes);
-                        uint64_t* bar = &ctl.full[stage];
-                        mbar_expect(bar, (uint32_t)(v_rows * U_CHUNK * 2 + slot.n * U_ROW * 2));
+                if (!behind) {
+                    wait_for_front();
+                    asm volatile("fence.proxy.async.global;" ::: "memory");
+                }
+                HeadPacks packs(a, row_tile);
+                HeadSlot slot[MAX_PACK];
+                int chunk[MAX_PACK], u_bytes;
+                while (const int n = packs.next(slot, chunk, &u_bytes)) {
+                    if (!take()) break;
+                    const uint32_t dst = base + (uint32_t)(stage * a.stage_bytes);
+                    uint64_t* bar = &ctl.full[stage];
+                    mbar_expect(bar, (uint32_t)(n * v_rows * a.u_cols * 2 + u_bytes));
+                    uint32_t u_dst = dst + A_BYTES;
+#pragma unroll
+                    for (int i = 0; i < MAX_PACK; i++) {
+                        if (i >= n) continue;
+                        const uint32_t b_dst = dst + (uint32_t)(i * VT * a.u_cols * 2);
                         if (v_rows == VT) {
-                            tma_3d(dst, &maps.b, c * U_CHUNK, v0, slot.adapter, bar);
+                            tma_3d(b_dst, &maps.b, chunk[i] * a.u_cols, v0, slot[i].adapter, bar);
                         } else {
                             for (int r = 0; r < v_rows; r += UNIT)
-                                tma_3d(dst + r * U_CHUNK * 2, &maps.b16, c * U_CHUNK, v0 + r, slot.adapter, bar);
+                                tma_3d(b_dst + r * a.u_cols * 2, &maps.b16, chunk[i] * a.u_cols, v0 + r, slot[i].adapter, bar);
                         }
-                        for (int r = 0; r < slot.n; r += WINDOW)
-                            tma_2d(dst + A_BYTES + r * U_ROW * 2, &maps.u, 0, c * a.u_chunk_rows + slot.u_row + r, bar);
-                        advance();
+                        for (int r = 0; r < slot[i].n; r += a.u_box)
+                            tma_2d(u_dst + r * a.u_cols * 4, &maps.u, 0, chunk[i] * a.u_rows + slot[i].u_row + r, bar);
+                        u_dst += (uint32_t)(slot[i].n * a.u_cols * 4);
                     }
+                    advance();
                 }
             }
             // every copy has landed before the CTA may end, whether its stage was used or not
@@ -299,12 +369,11 @@ __global__ void __launch_bounds__(HEAD_NT, 1) head_rows_kernel(const HeadArgs a,
             }
         }
         __syncwarp();
-    } else if (warp == 5) {
+    } else if (warp == WRITERS / 32 + 1) {
         if (lane == 0) {
-            int stage = 0, it = 0;
+            int stage = 0, round = 0;
             uint32_t phase = 0;
             bool ok = true;
-            if (a.slots_on) pdl_wait();  // the slots come from the kernel in front
             auto take = [&]() {
                 ok = head_wait(&ctl.full[stage], phase, &ctl.abort);
                 tmem_fence_after();
@@ -314,46 +383,64 @@ __global__ void __launch_bounds__(HEAD_NT, 1) head_rows_kernel(const HeadArgs a,
                 mma_commit(&ctl.empty[stage]);
                 if (++stage == a.stages) stage = 0, phase ^= 1;
             };
-            const uint32_t shape = E4M3 ? shape_e4m3(a.tile_cols) : shape_bf16(a.tile_cols);
-            for (; ok && tiles.next(&v0, &v_rows, &row_tile); it++) {
-                const int buf = it & 1;
-                ok = head_wait(&ctl.acc_empty[buf], ((it >> 1) & 1) ^ 1, &ctl.abort);
-                if (!ok) break;
+            uint32_t acc = 0;
+            auto begin_round = [&]() {
+                ok = head_wait(&ctl.acc_empty[round & 1], ((round >> 1) & 1) ^ 1, &ctl.abort);
                 tmem_fence_after();
-                const uint32_t acc = tmem + acc_of[buf];
-                // the slots' windows cover a tile in part only: zero times zero first
-                if (zero_first)
-                    mma_bf16(acc + slot_acc, operand<SWIZZLE_32>(zeros), operand<SWIZZLE_32>(zeros), shape_bf16(a.tile_cols), false);
+                acc = tmem + (uint32_t)(round & 1) * MAX_COLS;
+                return ok;
+            };
+            auto end_round = [&]() { mma_commit(&ctl.acc_full[round++ & 1]); };
+            const uint32_t shape = E4M3 ? shape_e4m3(a.tile_cols) : shape_bf16(a.tile_cols);
+            const uint64_t wide = operand_format(128), zero = operand(operand_format(32), zeros);
+            const uint64_t b_format = operand_format(a.u_cols * 2), u_format = operand_format(a.u_cols * 4);
+            while (ok && tiles.next(&v0, &v_rows, &row_tile)) {
                 for (int s = 0; s < a.w_steps; s++) {
+                    const bool first = s % ROUND == 0;
+                    if (first && !begin_round()) break;
                     if (!take()) break;
                     const uint32_t src = base + (uint32_t)(stage * a.stage_bytes);
 #pragma unroll
                     for (int k = 0; k < STEP_BYTES; k += 32) {
-                        const uint64_t wd = operand<SWIZZLE_128>(src + k), xd = operand<SWIZZLE_128>(src + A_BYTES + k);
-                        if (E4M3) mma_e4m3(acc, wd, xd, shape, s > 0 || k > 0);
-                        else mma_bf16(acc, wd, xd, shape, s > 0 || k > 0);
+                        const uint64_t wd = operand(wide, src + k), xd = operand(wide, src + A_BYTES + k);
+                        if (E4M3) mma_e4m3(acc, wd, xd, shape, !first || k > 0);
+                        else mma_bf16(acc, wd, xd, shape, !first || k > 0);
+                    }
+                    advance();
+                    if (s % ROUND == ROUND - 1 || s == a.w_steps - 1) {
+                        if (!(a.slots_on && !own_round && s == a.w_steps - 1)) end_round();
+                    }
+                }
+                if (!ok || !a.slots_on) continue;
+                wait_for_front();
+                HeadPacks packs(a, row_tile);
+                if (own_round) {
+                    if (packs.at == packs.end) continue;
+                    if (!begin_round()) break;
+                    // the slots' windows may cover a tile in part only: zero times zero first
+                    mma_bf16(acc, zero, zero, shape_bf16(a.tile_cols), false);
+                }
+                HeadSlot slot[MAX_PACK];
+                int chunk[MAX_PACK], u_bytes;
+                while (const int n = packs.next(slot, chunk, &u_bytes)) {
+                    if (!take()) break;
+                    const uint32_t src = base + (uint32_t)(stage * a.stage_bytes);
+                    uint32_t u_src = src + A_BYTES;
+#pragma unroll
+                    for (int i = 0; i < MAX_PACK; i++) {
+                        if (i >= n) continue;
+                        const uint32_t d = acc + (uint32_t)slot[i].col, n_shape = shape_bf16(slot[i].n);
+                        const uint32_t b_src = src + (uint32_t)(i * VT * a.u_cols * 2);
+                        for (int k = 0; k < a.u_cols && chunk[i] * a.u_cols + k < a.rank; k += 16) {
+                            const uint64_t bd = operand(b_format, b_src + k * 2);
+                            mma_bf16(d, bd, operand(u_format, u_src + k * 2), n_shape, true);
+                            mma_bf16(d, bd, operand(u_format, u_src + (a.u_cols + k) * 2), n_shape, true);
+                        }
+                        u_src += (uint32_t)(slot[i].n * a.u_cols * 4);
                     }
                     advance();
                 }
-                if (ok && a.slots_on) {
-                    const int end = a.tile_first[row_tile + 1];
-                    for (int i = a.tile_first[row_tile]; i < end && ok; i++) {
-                        const HeadSlot slot = a.slots[i];
-                        const uint32_t d = acc + slot_acc + (uint32_t)slot.col, n_shape = shape_bf16(slot.n);
-                        for (int c = 0; c < a.chunks; c++) {
-                            if (!take()) break;
-                            const uint32_t src = base + (uint32_t)(stage * a.stage_bytes);
-                            const int steps = (min(U_CHUNK, a.rank - c * U_CHUNK) + 15) / 16;
-                            for (int k = 0; k < steps; k++) {
-                                const uint64_t bd = operand<SWIZZLE_64>(src + k * 32);
-                                mma_bf16(d, bd, operand<SWIZZLE_128>(src + A_BYTES + k * 32), n_shape, true);
-                                mma_bf16(d, bd, operand<SWIZZLE_128>(src + A_BYTES + U_CHUNK * 2 + k * 32), n_shape, true);
-                            }
-                            advance();
-                        }
-                    }
-                }
-                if (ok) mma_commit(&ctl.acc_full[buf]);
+                if (ok) end_round();
             }
             if (!ok) {  // what was issued ends before tensor memory is given back
                 mma_commit(&ctl.drain);
@@ -362,67 +449,95 @@ __global__ void __launch_bounds__(HEAD_NT, 1) head_rows_kernel(const HeadArgs a,
         }
         __syncwarp();
     } else {
+        // a warp reads the 32 lanes of tensor memory that its number allows, and every other sixteen columns of them
+        const int quarter = warp & 3, half = warp >> 2;
+        const int w_rounds = (a.w_steps + ROUND - 1) / ROUND;
         bool ok = true;
-        pdl_wait();
-        for (int it = 0; ok && tiles.next(&v0, &v_rows, &row_tile); it++) {
-            const int buf = it & 1, place0 = row_tile * a.tile_cols, cols = min(a.tile_cols, a.rows - place0);
-            for (int c = threadIdx.x; c < a.tile_cols; c += 128) {
-                const int row = c < cols ? (a.perm ? a.perm[place0 + c] : place0 + c) : 0;
-                ctl.row_of[c] = row;
+        int round = 0;
+        if (a.sorted) wait_for_front();
+        while (ok && tiles.next(&v0, &v_rows, &row_tile)) {
+            const int place0 = row_tile * a.tile_cols, cols = min(a.tile_cols, a.rows - place0);
+            {
+                const int c = threadIdx.x;
+                const int row = c < cols ? (a.sorted ? a.perm[place0 + c] : place0 + c) : 0;
+                ctl.out_of[c] = row * a.out_stride * OUT_BYTES;
+                if (a.base) ctl.base_of[c] = row * a.base_stride * OUT_BYTES;
                 if (E4M3 && a.w_steps) ctl.scale_of[c] = a.x_scales[row];
             }
-            asm volatile("bar.sync 1, 128;" ::: "memory");
-            const int v = v0 + (int)threadIdx.x;
-            const bool mine = (int)threadIdx.x < v_rows && v < a.vocab;
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            const int v = v0 + quarter * 32 + lane;
+            const bool mine = quarter * 32 + lane < v_rows && v < a.vocab;
             const float w_scale = E4M3 && a.w_steps && mine ? a.w_scales[v] : 1.0f;
-            ok = head_wait(&ctl.acc_full[buf], (it >> 1) & 1, &ctl.abort);
-            ok = __all_sync(0xffffffffu, ok);
-            if (ok) {
-                tmem_fence_after();
-                const uint32_t acc = tmem + acc_of[buf] + ((uint32_t)(warp * 32) << 16);
-                for (int c0 = 0; c0 < cols; c0 += 16) {
-                    float d[16];
-                    tmem_load16(acc + c0, d);
-                    if (E4M3 && a.w_steps) {
+            float sum[GROUPS][16];
 #pragma unroll
-                        for (int i = 0; i < 16; i++) d[i] *= ctl.scale_of[c0 + i] * w_scale;
-                        if (a.slots_on) {
-                            float e[16];
-                            tmem_load16(acc + slot_acc + c0, e);
+            for (int j = 0; j < GROUPS; j++) {
 #pragma unroll
-                            for (int i = 0; i < 16; i++) d[i] += e[i];
-                        }
+                for (int i = 0; i < 16; i++) sum[j][i] = 0.0f;
+            }
+            if (a.base && mine) {
+                const char* from = static_cast<const char*>(a.base) + (long long)v * OUT_BYTES;
+#pragma unroll
+                for (int j = 0; j < GROUPS; j++) {
+                    const int c0 = j * 32 + half * 16;
+                    if (c0 < cols) {
+#pragma unroll
+                        for (int i = 0; i < 16; i++)  // (a column past the last reads its row 0: not stored)
+                            sum[j][i] = load1(reinterpret_cast<const Out*>(from + ctl.base_of[c0 + i]));
                     }
-                    if (mine) {
-                        if (a.base) {
-#pragma unroll
-                            for (int i = 0; i < 16; i++) {
-                                if (c0 + i >= cols) break;
-                                const long long at = (long long)ctl.row_of[c0 + i] * a.base_stride + v;
-                                d[i] += a.out_bf16 ? load1(static_cast<const bf16_raw*>(a.base) + at)
-                                                   : load1(static_cast<const float*>(a.base) + at);
-                            }
-                        }
-#pragma unroll
-                        for (int i = 0; i < 16; i++) {
-                            if (c0 + i >= cols) break;
-                            const long long at = (long long)ctl.row_of[c0 + i] * a.out_stride + v;
-                            if (a.out_bf16) store1(static_cast<bf16_raw*>(a.out) + at, d[i]);
-                            else store1(static_cast<float*>(a.out) + at, d[i]);
-                        }
-                    }
-                    __syncwarp();
                 }
-                tmem_fence_before();
+            }
+            int rounds = w_rounds;
+            if (own_round) {
+                wait_for_front();
+                rounds += a.tile_first[row_tile] < a.tile_first[row_tile + 1];
+            }
+            for (int r = 0; r < rounds && ok; r++, round++) {
+                // one lane of a warp watches the barrier
+                int landed = 1;
+                if (lane == 0) landed = head_wait(&ctl.acc_full[round & 1], (round >> 1) & 1, &ctl.abort);
+                ok = __shfl_sync(0xffffffffu, landed, 0);
+                if (ok) {
+                    tmem_fence_after();
+                    const uint32_t acc = tmem + (uint32_t)(round & 1) * MAX_COLS + ((uint32_t)(quarter * 32) << 16);
+                    const bool scaled = E4M3 && r < w_rounds;
+#pragma unroll
+                    for (int j = 0; j < GROUPS; j++) {
+                        const int c0 = j * 32 + half * 16;
+                        if (c0 < cols) {
+                            float d[16];
+                            tmem_load16(acc + c0, d);
+                            if (scaled) {
+#pragma unroll
+                                for (int i = 0; i < 16; i++) d[i] *= ctl.scale_of[c0 + i] * w_scale;
+                            }
+#pragma unroll
+                            for (int i = 0; i < 16; i++) sum[j][i] += d[i];
+                        }
+                    }
+                    tmem_fence_before();
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&ctl.acc_empty[round & 1]);
+            }
+            if (ok && mine) {
+                char* to = static_cast<char*>(a.out) + (long long)v * OUT_BYTES;
+#pragma unroll
+                for (int j = 0; j < GROUPS; j++) {
+                    const int c0 = j * 32 + half * 16;
+                    if (c0 < cols) {
+#pragma unroll
+                        for (int i = 0; i < 16; i++)
+                            if (c0 + i < cols) store1(reinterpret_cast<Out*>(to + ctl.out_of[c0 + i]), sum[j][i]);
+                    }
+                }
             }
             __syncwarp();
-            if (lane == 0) mbar_arrive(&ctl.acc_empty[buf]);
-            ok = epilogue_agree(ok);  // the tables are free, and the four warps go on together or not at all
+            ok = writers_agree(ok);  // the tables are free, and the warps go on together or not at all
         }
     }
     __syncthreads();
     if (threadIdx.x == 0 && ctl.abort && a.status) atomicOr(a.status, MANTLE_SAMPLE_STATUS_TIMEOUT);
-    if (warp == 5) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    if (warp == WRITERS / 32 + 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
 }
 
 }  // namespace
