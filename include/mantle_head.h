@@ -98,7 +98,7 @@ int mantleCudaNormRows(const MantleNormBatch* batch, mantleCudaStream_t stream);
  *   weight       [vocab][weight_stride] of `dtype`; starts on 16 bytes, weight_stride a multiple of 16 bytes
  *   base         [rows][base_stride] of out_dtype, instead of weight
  *   adapter_a    [n_adapters][rank][hidden] bfloat16, contiguous, on 16 bytes
- *   adapter_b    [n_adapters][vocab][rank] bfloat16, contiguous, on 16 bytes
+ *   adapter_b    what mantleCudaAdapterPack made of [n_adapters][vocab][rank] bfloat16; on 128 bytes
  *   adapter_gain [n_adapters] float32, or NULL: ones
  *   adapter_ids  [rows] int32, on the device: may change between launches, and between replays of a graph
  *   rank         a multiple of 8, up to MANTLE_HEAD_MAX_RANK; adapters of smaller rank are padded with zeros
@@ -109,8 +109,8 @@ int mantleCudaNormRows(const MantleNormBatch* batch, mantleCudaStream_t stream);
  *                kernel ran out (two seconds; the output is then not valid)
  *
  * Sums are float32; between the adapter's two products a value is held in two bfloat16 (16 bits of
- * mantissa).  The factors of all adapters have to be finite: rows are computed sixteen side by side, and an
- * infinity in one adapter's `b` makes NaN in rows beside those that use it.
+ * mantissa).  The factors of all adapters have to be finite: rows of several adapters share a step of the tensor
+ * cores, and an infinity in one adapter's `b` makes NaN in rows beside those that use it.
  *
  * `workspace`: mantleCudaHeadWorkspaceBytes() bytes on 256 bytes, needed with adapters or where hidden_rows do
  * not start on 16 bytes each, else NULL is fine.  Its contents mean nothing between calls; two calls that may
@@ -144,6 +144,14 @@ typedef struct MantleHeadBatch {
     int32_t rank;
     int32_t reserved;
 } MantleHeadBatch;
+
+/*
+ * Lays `b` of n adapters, [n][vocab][rank] bfloat16, contiguous and on 16 bytes, out as mantleCudaHeadRows reads it,
+ * once, when they are loaded.  An adapter's part of `packed` (on 128 bytes) is mantleCudaAdapterPackBytes(1, ...) bytes
+ * long, and n of them stand one after the other, so that one can be replaced.
+ */
+int mantleCudaAdapterPackBytes(int n, int vocab, int rank, size_t* bytes);
+int mantleCudaAdapterPack(const void* b, int n, int vocab, int rank, void* packed, mantleCudaStream_t stream);
 
 int mantleCudaHeadRows(const MantleHeadBatch* batch, void* workspace, size_t workspace_bytes,
                        mantleCudaStream_t stream);

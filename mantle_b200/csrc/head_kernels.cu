@@ -34,6 +34,11 @@ namespace {
 constexpr int kInvalid = (int)cudaErrorInvalidValue;
 constexpr int kMaxHeadHidden = 65536;
 constexpr int kMaxHeadRows = 1 << 20;
+// From how many rows on two CTAs share a tile.  (TODO figures)
+constexpr int PAIR_ROWS = 64;
+
+// The packed B of an adapter covers whole tiles of a pair.
+int padded_vocab(int vocab) { return (vocab + 2 * VT - 1) / (2 * VT) * (2 * VT); }
 
 int refuse(const char* why) {
     mantle_internal_set_last_error(why);
@@ -105,7 +110,7 @@ const char* head_fault(const MantleHeadBatch* b) {
         if (!b->adapter_a || !b->adapter_b || !b->adapter_ids) return "head: adapters need adapter_a, adapter_b and adapter_ids";
         if (b->rank <= 0 || b->rank > MANTLE_HEAD_MAX_RANK || b->rank % 8)
             return "head: rank must be a multiple of 8, up to MANTLE_HEAD_MAX_RANK";
-        if (!on(b->adapter_a, 16) || !on(b->adapter_b, 16)) return "head: adapter_a and adapter_b must start on 16 bytes";
+        if (!on(b->adapter_a, 16) || !on(b->adapter_b, 128)) return "head: adapter_a must start on 16 bytes, adapter_b on 128";
     } else if (b->base) {
         return "head: base without adapters";
     }
@@ -117,7 +122,8 @@ struct HeadLayout {
     bool eight, adapters;
     bool sorted;  // rows in the order of their adapters
     bool copied;  // x is read from the workspace's copy
-    int tile_cols, row_tiles, v_tiles, w_steps, u_cols, chunks, slot_bound, box_bound, u_rows;
+    bool pair;    // two CTAs to a tile
+    int tile_cols, row_tiles, v_tiles, w_steps, chunks, slot_bound, box_bound, u_rows;
     int stages, stage_bytes, grid;
     size_t smem;
     size_t perm, slots, boxes, tile_first, n_boxes, u, xs, total;
@@ -132,18 +138,19 @@ HeadLayout head_layout(const MantleHeadBatch* b) {
     const bool weight = b->weight != nullptr;
     l.sorted = l.adapters && b->rows > HERE_ROWS;
     l.copied = weight && (l.sorted || !aligned);  // beside a projection x is only read by the shrink kernels
+    l.pair = b->rows > PAIR_ROWS;
+    const int ctas = l.pair ? 2 : 1, step = 16 * ctas;
     l.row_tiles = (b->rows + MAX_COLS - 1) / MAX_COLS;
-    l.tile_cols = ((b->rows + l.row_tiles - 1) / l.row_tiles + WINDOW - 1) / WINDOW * WINDOW;
+    l.tile_cols = ((b->rows + l.row_tiles - 1) / l.row_tiles + step - 1) / step * step;
     l.row_tiles = (b->rows + l.tile_cols - 1) / l.tile_cols;
-    l.v_tiles = (b->vocab + VT - 1) / VT;
+    l.v_tiles = (b->vocab + VT * ctas - 1) / (VT * ctas);
     l.w_steps = weight ? (int)((b->hidden * e + STEP_BYTES - 1) / STEP_BYTES) : 0;
-    const int sms = device_info().sms;
-    l.grid = l.row_tiles == 1 ? std::min(sms, (b->vocab + UNIT - 1) / UNIT)
-                              : (int)std::min<long long>(sms, (long long)l.v_tiles * l.row_tiles);
+    const long long work = l.row_tiles == 1 ? (b->vocab + UNIT * ctas - 1) / (UNIT * ctas) : (long long)l.v_tiles * l.row_tiles;
+    l.grid = (int)std::min<long long>(device_info().sms / ctas, work) * ctas;
     const bool own_round = l.adapters && (l.eight || !weight);
     const size_t fixed = 1024 + sizeof(HeadCtl) + (own_round ? ZERO_BYTES : 0);
     // Adapters on the whole tile: room for four windows of u, as far as that is no more than W's share of the stage.
-    const int x_bytes = l.tile_cols * STEP_BYTES;
+    const int x_bytes = l.tile_cols / ctas * STEP_BYTES;
     l.stage_bytes = A_BYTES + (l.adapters && !l.sorted ? std::max(x_bytes, std::min(2 * x_bytes, A_BYTES)) : x_bytes);
     l.stages = (int)std::min<size_t>(MAX_STAGES, ((size_t)232448 - fixed) / (size_t)l.stage_bytes);
     l.smem = fixed + (size_t)l.stages * (size_t)l.stage_bytes;
@@ -154,14 +161,12 @@ HeadLayout head_layout(const MantleHeadBatch* b) {
         return at;
     };
     if (l.adapters) {
-        l.u_cols = b->rank <= 16 ? 16 : 32;
-        l.chunks = (b->rank + l.u_cols - 1) / l.u_cols;
+        l.chunks = (b->rank + U_RANKS - 1) / U_RANKS;
         l.slot_bound = std::min(b->rows, b->n_adapters);
         if (l.sorted) {
-            // a piece per adapter in use and one per cut; each box holds a row at least, and a piece of n rows touches
-            // at most n / 16 + 2 boxes
-            const int cuts = l.row_tiles * ((l.tile_cols + SLOT_COLS - 1) / SLOT_COLS);
-            l.slot_bound = std::min(b->rows, l.slot_bound + cuts);
+            // a piece per adapter in use and one per tile's end; each box holds a row at least, and a piece of n rows
+            // touches at most n / WINDOW + 2 boxes
+            l.slot_bound = std::min(b->rows, l.slot_bound + l.row_tiles);
             l.box_bound = std::min(b->rows, b->rows / WINDOW + 2 * l.slot_bound);
             l.perm = take((size_t)b->rows * 4);
             l.boxes = take((size_t)l.box_bound * sizeof(HeadBox));
@@ -170,7 +175,7 @@ HeadLayout head_layout(const MantleHeadBatch* b) {
         l.u_rows = l.sorted ? l.box_bound * WINDOW : l.slot_bound * l.tile_cols;
         l.slots = take((size_t)l.slot_bound * sizeof(HeadSlot));
         l.tile_first = take((size_t)(l.row_tiles + 1) * 4);
-        l.u = take((size_t)l.chunks * (size_t)l.u_rows * (size_t)l.u_cols * 4);
+        l.u = take((size_t)l.chunks * (size_t)l.u_rows * U_BYTES);
     }
     if (l.copied) l.xs = take((size_t)b->rows * (size_t)b->hidden * e);
     return l;
@@ -209,30 +214,32 @@ bool encode_rows(CUtensorMap* m, const void* p, bool eight, long long rows, long
     const cuuint32_t box[2] = {(cuuint32_t)(STEP_BYTES / (eight ? 1 : 2)), (cuuint32_t)box_rows};
     return encode(m, p, eight, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
-bool encode_u(CUtensorMap* m, const void* p, const HeadLayout& l, int box_rows) {
-    const cuuint64_t dims[2] = {(cuuint64_t)l.u_cols * 2, (cuuint64_t)l.chunks * (cuuint64_t)l.u_rows}, strides[1] = {(cuuint64_t)l.u_cols * 4};
-    const cuuint32_t box[2] = {(cuuint32_t)l.u_cols * 2, (cuuint32_t)box_rows};
-    return encode(m, p, false, 2, dims, strides, box, l.u_cols == 16 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B);
-}
-bool encode_b(CUtensorMap* m, const MantleHeadBatch* b, const HeadLayout& l, int box_rows) {
-    const cuuint64_t dims[3] = {(cuuint64_t)b->rank, (cuuint64_t)b->vocab, (cuuint64_t)b->n_adapters};
-    const cuuint64_t strides[2] = {(cuuint64_t)b->rank * 2, (cuuint64_t)b->rank * 2 * (cuuint64_t)b->vocab};
-    const cuuint32_t box[3] = {(cuuint32_t)l.u_cols, (cuuint32_t)box_rows, 1};
-    return encode(m, b->adapter_b, false, 3, dims, strides, box, l.u_cols == 16 ? CU_TENSOR_MAP_SWIZZLE_32B : CU_TENSOR_MAP_SWIZZLE_64B);
+// Plain 128-byte rows (packed B, u): [d2][d1] of them, `box_rows` a copy.
+bool encode_plain(CUtensorMap* m, const void* p, long long d1, long long d2, int box_rows) {
+    const cuuint64_t dims[3] = {64, (cuuint64_t)d1, (cuuint64_t)d2}, strides[2] = {128, 128 * (cuuint64_t)d1};
+    const cuuint32_t box[3] = {64, (cuuint32_t)box_rows, 1};
+    return encode(m, p, false, d2 ? 3 : 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
 template <class... Args>
-int launch(void (*kern)(Args...), dim3 grid, int threads, size_t smem, cudaStream_t stream, bool dependent, Args... args) {
+int launch(void (*kern)(Args...), dim3 grid, int threads, size_t smem, cudaStream_t stream, bool dependent, bool pair, Args... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = dim3((unsigned)threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchAttribute attr[2];
     cfg.attrs = attr;
-    cfg.numAttrs = dependent ? 1 : 0;
+    if (dependent) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (pair) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        attr[cfg.numAttrs].val.clusterDim.x = 2;
+        attr[cfg.numAttrs].val.clusterDim.y = 1;
+        attr[cfg.numAttrs++].val.clusterDim.z = 1;
+    }
     return (int)cudaLaunchKernelEx(&cfg, kern, args...);
 }
 
@@ -242,13 +249,13 @@ int launch_head_as(const HeadArgs& a, const HeadMaps& maps, const HeadLayout& l,
     const auto kern = head_rows_kernel<E4M3, OUT16, GROUPS>;
     const int rc = ensure_smem(kern, l.smem, granted);
     if (rc) return rc;
-    return launch<HeadArgs, HeadMaps>(kern, dim3((unsigned)l.grid), HEAD_NT, l.smem, stream, l.adapters || l.copied, a, maps);
+    return launch<HeadArgs, HeadMaps>(kern, dim3((unsigned)l.grid), HEAD_NT, l.smem, stream, l.adapters || l.copied, l.pair, a, maps);
 }
 
 template <bool E4M3, bool OUT16>
 int launch_head(const HeadArgs& a, const HeadMaps& maps, const HeadLayout& l, cudaStream_t stream) {
     if (l.tile_cols <= 32) return launch_head_as<E4M3, OUT16, 1>(a, maps, l, stream);
-    if (l.tile_cols <= 64) return launch_head_as<E4M3, OUT16, 2>(a, maps, l, stream);
+    if (!l.pair) return launch_head_as<E4M3, OUT16, 2>(a, maps, l, stream);
     if (l.tile_cols <= 128) return launch_head_as<E4M3, OUT16, 4>(a, maps, l, stream);
     return launch_head_as<E4M3, OUT16, 8>(a, maps, l, stream);
 }
@@ -284,6 +291,26 @@ extern "C" int mantleCudaNormRows(const MantleNormBatch* b, mantleCudaStream_t s
                      (quant ? on(b->out, 8) && b->out_stride % 8 == 0 : rows_on_16(b->out, b->out_stride));
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
     return b->dtype == MANTLE_DTYPE_F32 ? launch_norm<float>(a, quant, vec, stream) : launch_norm<bf16_raw>(a, quant, vec, stream);
+}
+
+extern "C" int mantleCudaAdapterPackBytes(int n, int vocab, int rank, size_t* bytes) {
+    if (!bytes || n <= 0 || n > MANTLE_HEAD_MAX_ADAPTERS || vocab <= 0 || vocab > MANTLE_SAMPLE_MAX_VOCAB || rank <= 0 ||
+        rank > MANTLE_HEAD_MAX_RANK || rank % 8)
+        return refuse("adapter pack: n, vocab or rank is out of range");
+    *bytes = (size_t)n * ((rank + U_RANKS - 1) / U_RANKS) * (size_t)padded_vocab(vocab) * U_RANKS * 2;
+    return 0;
+}
+
+extern "C" int mantleCudaAdapterPack(const void* b, int n, int vocab, int rank, void* packed, mantleCudaStream_t stream_) {
+    size_t bytes = 0;
+    const int rc = mantleCudaAdapterPackBytes(n, vocab, rank, &bytes);
+    if (rc) return rc;
+    if (!b || !packed || !on(b, 16) || !on(packed, 128))
+        return refuse("adapter pack: b must start on 16 bytes, packed on 128");
+    const int grid = (int)std::min<size_t>((bytes / 16 + 255) / 256, (size_t)device_info().sms * 16);
+    adapter_pack_kernel<<<grid, 256, 0, static_cast<cudaStream_t>(stream_)>>>(
+        static_cast<const bf16_raw*>(b), n, vocab, rank, padded_vocab(vocab), static_cast<bf16_raw*>(packed));
+    return (int)cudaGetLastError();
 }
 
 extern "C" int mantleCudaHeadWorkspaceBytes(const MantleHeadBatch* b, size_t* bytes) {
@@ -322,10 +349,11 @@ extern "C" int mantleCudaHeadRows(const MantleHeadBatch* b, void* workspace, siz
     a.slots_on = l.adapters;
     a.sorted = l.sorted;
     a.copied = l.copied;
-    a.rank = b->rank;
-    a.u_cols = l.u_cols;
+    a.chunks = l.chunks;
     a.u_rows = l.u_rows;
-    a.u_box = l.sorted ? WINDOW : l.tile_cols;
+    a.u_box = l.sorted ? WINDOW / 2 : l.tile_cols / (l.pair ? 2 : 1);
+    const int padded = padded_vocab(b->vocab);
+    a.b_rows = padded / 4;
     a.stages = l.stages;
     a.stage_bytes = l.stage_bytes;
     a.x_scales = b->hidden_scales;
@@ -349,7 +377,6 @@ extern "C" int mantleCudaHeadRows(const MantleHeadBatch* b, void* workspace, siz
     p.vec = on(b->hidden_rows, 16) && b->hidden_stride * e % 16 == 0;
     p.n_adapters = b->n_adapters;
     p.rank = b->rank;
-    p.u_cols = l.u_cols;
     p.u_rows = l.u_rows;
     p.tile_cols = l.tile_cols;
     p.row_tiles = l.row_tiles;
@@ -373,27 +400,30 @@ extern "C" int mantleCudaHeadRows(const MantleHeadBatch* b, void* workspace, siz
     HeadMaps maps;
     memset(&maps, 0, sizeof maps);
     bool ok = true;
+    const int x_rows = l.tile_cols / (l.pair ? 2 : 1);
     if (b->weight) {
         ok = ok && encode_rows(&maps.w, b->weight, l.eight, b->vocab, b->hidden, b->weight_stride * e, VT);
         ok = ok && encode_rows(&maps.w16, b->weight, l.eight, b->vocab, b->hidden, b->weight_stride * e, UNIT);
-        ok = ok && (p.xs ? encode_rows(&maps.x, p.xs, l.eight, b->rows, b->hidden, b->hidden * e, l.tile_cols)
-                         : encode_rows(&maps.x, b->hidden_rows, l.eight, b->rows, b->hidden, b->hidden_stride * e, l.tile_cols));
+        ok = ok && (p.xs ? encode_rows(&maps.x, p.xs, l.eight, b->rows, b->hidden, b->hidden * e, x_rows)
+                         : encode_rows(&maps.x, b->hidden_rows, l.eight, b->rows, b->hidden, b->hidden_stride * e, x_rows));
     }
     if (l.adapters) {
-        ok = ok && encode_b(&maps.b, b, l, VT) && encode_b(&maps.b16, b, l, UNIT);
-        ok = ok && encode_u(&maps.u, p.u, l, a.u_box);
+        const long long per_adapter = (long long)l.chunks * a.b_rows;
+        ok = ok && encode_plain(&maps.b, b->adapter_b, per_adapter, b->n_adapters, VT / 4);
+        ok = ok && encode_plain(&maps.b16, b->adapter_b, per_adapter, b->n_adapters, UNIT / 4);
+        ok = ok && encode_plain(&maps.u, p.u, (long long)l.chunks * l.u_rows / 2, 0, a.u_box / 2);
     }
     if (!ok) return refuse("head: the driver refused a tensor map");
 
     int rc = 0;
     if (l.sorted) {
-        rc = launch<HeadPrep>(head_sort_kernel, dim3(1), SORT_NT, ((size_t)b->n_adapters + 1) * 4, stream, false, p);
+        rc = launch<HeadPrep>(head_sort_kernel, dim3(1), SORT_NT, ((size_t)b->n_adapters + 1) * 4, stream, false, false, p);
         if (rc) return rc;
     }
     if (l.adapters || l.copied) {
         const dim3 grid((unsigned)(p.units + p.copy_ctas), (unsigned)(l.adapters ? b->rank / 8 : 1));
-        rc = l.sorted ? launch<HeadPrep>(head_shrink_kernel, grid, SHRINK_NT, 0, stream, true, p)
-                      : launch<HeadPrep>(head_shrink_here_kernel, grid, SHRINK_NT, 0, stream, false, p);
+        rc = l.sorted ? launch<HeadPrep>(head_shrink_kernel, grid, SHRINK_NT, 0, stream, true, false, p)
+                      : launch<HeadPrep>(head_shrink_here_kernel, grid, SHRINK_NT, 0, stream, false, false, p);
         if (rc) return rc;
     }
     if (b->out_dtype == MANTLE_DTYPE_BF16)

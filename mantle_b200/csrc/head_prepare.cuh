@@ -20,8 +20,9 @@
 
 namespace {
 
-constexpr int WINDOW = 16;         // columns of D come in sixteens
-constexpr int SLOT_COLS = 128;     // sorted: a slot's window lies within an aligned run of 128 columns of its tile
+constexpr int WINDOW = 32;         // sorted: windows start and end on a multiple of 32 columns of their tile
+constexpr int U_RANKS = 16;        // ranks of one step of the tensor cores: a chunk
+constexpr int U_BYTES = 4 * U_RANKS;  // a row of u of one chunk: sixteen leading parts and sixteen remainders
 constexpr int HERE_ROWS = 128;
 constexpr int SORT_NT = 1024;
 constexpr int SHRINK_NT = 512;
@@ -32,7 +33,7 @@ constexpr int SHRINK_WARPS = SHRINK_NT / 32;
 struct __align__(16) HeadSlot {
     int adapter, col, n, u_row;
 };
-// Sixteen rows of u: sorted places [place, place + 16), of which [first, last) use the adapter.
+// WINDOW rows of u: sorted places [place, place + WINDOW), of which [first, last) use the adapter.
 struct __align__(16) HeadBox {
     int adapter, place, first, last;
 };
@@ -47,7 +48,6 @@ struct HeadPrep {
     long long x_stride;  // elements
     int rows, hidden, e4m3, vec;  // vec: rows of x start on 16 bytes
     int n_adapters, rank;
-    int u_cols;          // ranks of one step, 16 or 32: a row of u holds as many leading parts, then as many remainders
     int u_rows;          // rows of u of one chunk of ranks
     int tile_cols, row_tiles;
     int units, copy_ctas;  // CTAs of the shrink kernel: slots or boxes at most; and those that copy x
@@ -57,7 +57,7 @@ struct HeadPrep {
     HeadBox* boxes;
     int* tile_first;  // [row_tiles + 1] first slot of a tile
     int* n_boxes;     // [1]
-    bf16_raw* u;      // [chunks][u_rows][2 * u_cols]
+    bf16_raw* u;      // [chunks][u_rows / 8][4][8][8], see u_at
     void* xs;         // [rows][hidden] contiguous, sorted
 };
 
@@ -88,7 +88,7 @@ __device__ __forceinline__ int block_scan(int v, int* warp_sums, int* total) {
 }
 
 // One CTA: counts the rows of every adapter, gives each adapter its run of places (rows without one come
-// last), and cuts the runs into slots and boxes.  Shared memory: n_adapters + 1 counts.
+// last), and cuts the runs into slots, at the ends of tiles, and boxes.  Shared memory: n_adapters + 1 counts.
 __global__ void __launch_bounds__(SORT_NT) head_sort_kernel(const HeadPrep p) {
     extern __shared__ int bins[];  // [n_adapters + 1]: counts, then next free places, then ends of runs
     __shared__ int warp_sums[32];
@@ -116,15 +116,11 @@ __global__ void __launch_bounds__(SORT_NT) head_sort_kernel(const HeadPrep p) {
     }
     __syncthreads();  // bins[b] is now the end of run b, and its start the end of run b - 1
 
-    // A run is cut where a tile ends, and inside a tile at every 128 columns.
     int slot_carry = 0, box_carry = 0;
     for (int b0 = 0; b0 < n; b0 += SORT_NT) {
         const int b = b0 + tid;
         const int lo = b < n ? (b ? bins[b - 1] : 0) : 0, hi = b < n ? bins[b] : 0;
-        auto cut = [&](int at) {  // end of the piece that starts at place `at`
-            const int tile = at / p.tile_cols, col = at % p.tile_cols;
-            return min(hi, min((tile + 1) * p.tile_cols, tile * p.tile_cols + (col / SLOT_COLS + 1) * SLOT_COLS));
-        };
+        auto cut = [&](int at) { return min(hi, (at / p.tile_cols + 1) * p.tile_cols); };  // end of the piece that starts at `at`
         int n_slots = 0, n_boxes = 0;
         for (int at = lo; at < hi;) {
             const int end = cut(at), tile0 = at / p.tile_cols * p.tile_cols;
@@ -261,25 +257,33 @@ __device__ __forceinline__ float shrink16(const HeadPrep& p, int adapter, int j0
     return v;
 }
 
+// u lies in memory as the tensor cores read it from shared memory without swizzle: blocks of 8 rows by 8 values (16
+// bytes a row), four to a group of 8 rows -- leading parts of ranks 0-7 and 8-15 of the chunk, then the remainders --
+// so that any run of rows is one contiguous copy.
+__device__ __forceinline__ bf16_raw* u_at(const HeadPrep& p, int rank_at, int u_row) {
+    return p.u + ((long long)(rank_at / U_RANKS) * p.u_rows + (u_row & ~7)) * (U_BYTES / 2) +
+           (rank_at % U_RANKS / 8) * 64 + (u_row & 7) * 8 + rank_at % 8;
+}
+
 // v in two bfloat16: 16 bits of mantissa (an infinity or NaN stays in the leading part alone).  Where the rank ends
-// inside a step of sixteen, the thread of its last eight also writes the zeros behind them.
+// inside a chunk, the thread of its last eight also writes the zeros behind them.
 __device__ __forceinline__ void store_u(const HeadPrep& p, int rank_at, int u_row, float v) {
     const uint32_t hi = pack_bf16(v, 0.0f) & 0xffffu;
     const float rest = v - __uint_as_float(hi << 16);
     const uint32_t lo = (hi & 0x7f80u) == 0x7f80u ? 0u : pack_bf16(rest, 0.0f) & 0xffffu;
-    bf16_raw* u = p.u + ((long long)(rank_at / p.u_cols) * p.u_rows + u_row) * (2 * p.u_cols) + rank_at % p.u_cols;
+    bf16_raw* u = u_at(p, rank_at, u_row);
     u[0] = (bf16_raw)hi;
-    u[p.u_cols] = (bf16_raw)lo;
-    if (rank_at + 8 >= p.rank && p.rank % 16) {
-        u[8] = 0;
-        u[p.u_cols + 8] = 0;
+    u[128] = (bf16_raw)lo;
+    if (rank_at + 8 >= p.rank && p.rank % U_RANKS) {
+        u[64] = 0;
+        u[192] = 0;
     }
 }
 
 // Sorted form.  CTAs [0, units) x [0, rank / 8): eight ranks of one box.  CTAs from `units` on: the copy of x.
 __global__ void __launch_bounds__(SHRINK_NT) head_shrink_kernel(const HeadPrep p) {
     __shared__ float sums[SHRINK_WARPS][16][8];
-    __shared__ int rows[16];
+    __shared__ int rows[WINDOW];
     pdl_trigger();
     pdl_wait();
     if ((int)blockIdx.x >= p.units) {
@@ -289,14 +293,18 @@ __global__ void __launch_bounds__(SHRINK_NT) head_shrink_kernel(const HeadPrep p
     }
     if ((int)blockIdx.x >= *p.n_boxes) return;
     const HeadBox box = p.boxes[blockIdx.x];
-    if (threadIdx.x < 16) {
+    if (threadIdx.x < WINDOW) {
         const int at = box.place + (int)threadIdx.x;
         rows[threadIdx.x] = at >= box.first && at < box.last ? p.perm[at] : -1;
     }
     __syncthreads();
-    const int j0 = blockIdx.y * 8;
-    const float v = shrink16(p, box.adapter, j0, rows, sums);
-    if (threadIdx.x < 128) store_u(p, j0 + (int)(threadIdx.x & 7), (int)blockIdx.x * WINDOW + (int)(threadIdx.x >> 3), v);
+    const int j0 = blockIdx.y * 8, j = threadIdx.x & 7, i = threadIdx.x >> 3;
+    for (int r = 0; r < WINDOW; r += 16) {
+        const bool some = box.first < box.place + r + 16 && box.last > box.place + r;
+        const float v = some ? shrink16(p, box.adapter, j0, rows + r, sums) : 0.0f;
+        if (threadIdx.x < 128) store_u(p, j0 + j, (int)blockIdx.x * WINDOW + r + i, v);
+        __syncthreads();
+    }
 }
 
 // Form for up to HERE_ROWS rows.  CTAs [0, units) x [0, rank / 8): eight ranks of the rows of one adapter -- the
@@ -367,6 +375,24 @@ __global__ void __launch_bounds__(SHRINK_NT) head_shrink_here_kernel(const HeadP
         const float v = shrink16(p, adapter, j0, mine + i, sums);
         if (tid < 128 && i + (tid >> 3) < n) store_u(p, j0 + (tid & 7), u_row + mine[i + (tid >> 3)], v);
         __syncthreads();
+    }
+}
+
+// B of the adapters as the tensor cores read it, so that any run of 8 vocabulary rows of a chunk of 16 ranks is one
+// contiguous copy: [n][chunks][padded / 8][2][8][8], blocks of 8 vocabulary rows by 8 ranks; zeros behind the
+// vocabulary and the rank.  (From [vocab][rank] rows of 32 bytes the copies ran at a few requests a microsecond: 16
+// adapters of rank 16 cost 64 rows 58 us more than their bytes take.)  One thread, one row of a block.
+__global__ void __launch_bounds__(256) adapter_pack_kernel(const bf16_raw* b, int n, int vocab, int rank, int padded, bf16_raw* packed) {
+    const int chunks = (rank + U_RANKS - 1) / U_RANKS;
+    const long long total = (long long)n * chunks * padded * 2;
+    for (long long t = (long long)blockIdx.x * 256 + threadIdx.x; t < total; t += (long long)gridDim.x * 256) {
+        const int in_group = (int)(t % 16);
+        const long long group = t / 16;
+        const long long v = group % (padded / 8) * 8 + in_group % 8, above = group / (padded / 8);
+        const int k = (int)(above % chunks) * U_RANKS + in_group / 8 * 8;
+        uint4 w = make_uint4(0, 0, 0, 0);
+        if (v < vocab && k < rank) w = *reinterpret_cast<const uint4*>(b + (above / chunks * vocab + v) * rank + k);
+        reinterpret_cast<uint4*>(packed)[t] = w;
     }
 }
 

@@ -9,9 +9,15 @@
 // rows, whatever the number of rows.
 //
 // One CTA per SM, persistent over its tiles.  Warp 8 moves operands with TMA into a ring of stages (a stage: 128
-// rows of W, 128 bytes wide, and the same slice of x; or some adapters' B, 16 or 32 ranks wide, and their windows of
-// u), warp 9 issues tcgen05.mma from it, warps 0-7 read accumulators out of tensor memory, add them up in
-// registers and write the finished tile while the next one is computed.
+// rows of W, 128 bytes wide, and the same slice of x; or some adapters' B, 16 ranks wide, and their windows of u),
+// warp 9 issues tcgen05.mma from it, warps 0-7 read accumulators out of tensor memory, add them up in registers
+// and write the finished tile while the next one is computed.
+//
+// Pairs.  W comes from HBM once, but x from L2 for every 128 vocabulary rows: at 256 rows that is twice W's bytes,
+// and what L2 can hand out (about 10 TB/s) bounds the kernel long before HBM or the tensor cores do.  From 65 rows
+// on two CTAs therefore compute 256 vocabulary rows together (cta_group::2): each holds its own 128 rows of W and
+// of the accumulator, and half of x.  The even CTA of a pair issues the products; copies of both complete on its
+// barriers.
 //
 // Rounds.  A float32 accumulator in tensor memory is cut, not rounded, at every step, so its error grows with the
 // number of steps, always towards zero (measured with bfloat16 operands: 2.3e-7 of the result after 256 columns,
@@ -31,13 +37,14 @@ constexpr int STEP_BYTES = 128;    // bytes of a row that one stage holds
 constexpr int A_BYTES = VT * STEP_BYTES;
 constexpr int MAX_COLS = 256;
 constexpr int MAX_STAGES = 12;
-constexpr int UNIT = 16;           // vocabulary rows by which single-tile batches are shared out
+constexpr int UNIT = 16;           // vocabulary rows of a CTA by which single-tile batches are shared out
+constexpr int B_BYTES = VT * U_RANKS * 2;  // one adapter's B of one chunk and a whole tile
 constexpr int ROUND_BF16 = 8;      // steps of a round
 constexpr int ROUND_E4M3 = 64;
 constexpr int WRITERS = 256;       // threads that read accumulators and write results
 constexpr int HEAD_NT = WRITERS + 64;
-constexpr int ZERO_BYTES = MAX_COLS * 32;
-constexpr int MAX_PACK = 4;        // adapters' steps in one stage
+constexpr int ZERO_BYTES = VT * 32;
+constexpr int MAX_PACK = A_BYTES / B_BYTES;  // adapters' steps in one stage
 
 struct HeadCtl {
     uint64_t full[MAX_STAGES], empty[MAX_STAGES], acc_full[2], acc_empty[2], drain;
@@ -50,7 +57,8 @@ struct HeadCtl {
 struct HeadArgs {
     int rows, vocab, w_steps, tile_cols, row_tiles, v_tiles;
     int slots_on, sorted, copied;  // adapters; perm and x come from the kernel in front
-    int rank, u_cols, u_rows, u_box;  // u_box: rows of u of one copy
+    int chunks, u_rows, u_box;        // u_box: rows of u of one copy
+    int b_rows;                       // 128-byte rows of one chunk of an adapter's B
     int stages, stage_bytes;
     const int* perm;
     const HeadSlot* slots;
@@ -64,7 +72,7 @@ struct HeadArgs {
 };
 
 struct HeadMaps {
-    CUtensorMap w, w16, x, b, b16, u;
+    CUtensorMap w, w16, x, b, b16, u;  // (b, b16 and u: plain 128-byte rows)
 };
 
 // ---- the instructions
@@ -72,42 +80,81 @@ struct HeadMaps {
 __device__ __forceinline__ void mbar_expect(uint64_t* bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+// The address of `bar` in the pair's even CTA (PAIR), or in this one.
+template <bool PAIR>
+__device__ __forceinline__ uint32_t lead_bar(uint64_t* bar) {
+    uint32_t at = smem_u32(bar);
+    if (PAIR) asm volatile("mapa.shared::cluster.u32 %0, %0, 0;" : "+r"(at));
+    return at;
 }
-__device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
-    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-                 ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar)) : "memory");
+template <bool PAIR>
+__device__ __forceinline__ void lead_arrive(uint64_t* bar) {
+    if (PAIR) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(lead_bar<true>(bar)) : "memory");
+    else asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
-__device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
-    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
-                 ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar)) : "memory");
+// Copies to this CTA's shared memory that complete on a barrier of the pair's even CTA (bar: lead_bar's).
+template <bool PAIR>
+__device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+    if (PAIR)
+        asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                     ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
+    else
+        asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                     ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
+}
+template <bool PAIR>
+__device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+    if (PAIR)
+        asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                     ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
+    else
+        asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                     ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
 }
 
-// Shared-memory matrix descriptor of a K-major operand: rows of 128, 64 or 32 bytes, swizzled by the same
-// width, eight rows to a group and the groups one after the other.
-__device__ __forceinline__ uint64_t operand_format(int row_bytes) {
-    const uint64_t swizzle = row_bytes == 128 ? 2 : row_bytes == 64 ? 4 : 6;
-    return (uint64_t)1 << 16 | (uint64_t)(row_bytes * 8 >> 4) << 32 | (uint64_t)1 << 46 | swizzle << 61;
-}
+// Shared-memory matrix descriptors of K-major operands.  W and x: rows of 128 bytes, swizzled, 1024 bytes from eight
+// rows to the next eight.  B and u: blocks of 8 rows by 16 bytes, 128 bytes from one block of a row to the next, and
+// `group` bytes from eight rows to the next eight.
+constexpr uint64_t SWIZZLED_ROWS = (uint64_t)1 << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+__device__ constexpr uint64_t blocks(int group) { return (uint64_t)(128 >> 4) << 16 | (uint64_t)(group >> 4) << 32 | (uint64_t)1 << 46; }
 __device__ __forceinline__ uint64_t operand(uint64_t format, uint32_t addr) { return format | (uint64_t)((addr >> 4) & 0x3fff); }
-// Instruction descriptor: float32 accumulator, 128 x n; bfloat16 operands, or e4m3.
+// Instruction descriptor: float32 accumulator, 128 (a pair: 256) x n; bfloat16 operands, or e4m3.
+template <bool PAIR>
 __device__ __forceinline__ uint32_t shape_bf16(int n) {
-    return 1u << 4 | 1u << 7 | 1u << 10 | (uint32_t)(n >> 3) << 17 | (uint32_t)(VT >> 4) << 24;
+    return 1u << 4 | 1u << 7 | 1u << 10 | (uint32_t)(n >> 3) << 17 | (uint32_t)(VT * (PAIR ? 2 : 1) >> 4) << 24;
 }
+template <bool PAIR>
 __device__ __forceinline__ uint32_t shape_e4m3(int n) {
-    return 1u << 4 | (uint32_t)(n >> 3) << 17 | (uint32_t)(VT >> 4) << 24;
+    return 1u << 4 | (uint32_t)(n >> 3) << 17 | (uint32_t)(VT * (PAIR ? 2 : 1) >> 4) << 24;
 }
-__device__ __forceinline__ void mma_bf16(uint32_t d, uint64_t a, uint64_t b, uint32_t shape, bool add) {
-    asm volatile("{.reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;}"
-                 ::"r"(d), "l"(a), "l"(b), "r"(shape), "r"((int)add) : "memory");
+template <bool PAIR, bool E4M3>
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t shape, bool add) {
+#define MANTLE_MMA(GROUP, KIND)                                                                                          \
+    asm volatile("{.reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::" GROUP ".kind::" KIND " [%0], %1, %2, %3, p;}" \
+                 ::"r"(d), "l"(a), "l"(b), "r"(shape), "r"((int)add) : "memory")
+    if (PAIR && E4M3) MANTLE_MMA("2", "f8f6f4");
+    else if (PAIR) MANTLE_MMA("2", "f16");
+    else if (E4M3) MANTLE_MMA("1", "f8f6f4");
+    else MANTLE_MMA("1", "f16");
+#undef MANTLE_MMA
 }
-__device__ __forceinline__ void mma_e4m3(uint32_t d, uint64_t a, uint64_t b, uint32_t shape, bool add) {
-    asm volatile("{.reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;}"
-                 ::"r"(d), "l"(a), "l"(b), "r"(shape), "r"((int)add) : "memory");
-}
+// Arrives on `bar` -- of both CTAs of a pair -- when the products issued so far are done.
+template <bool PAIR>
 __device__ __forceinline__ void mma_commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+    if (PAIR)
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                     ::"r"(smem_u32(bar)), "h"((uint16_t)3) : "memory");
+    else
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+// All threads of the CTA, or of the pair.
+template <bool PAIR>
+__device__ __forceinline__ void sync_all() {
+    if (PAIR) {
+        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    } else {
+        __syncthreads();
+    }
 }
 __device__ __forceinline__ void tmem_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tmem_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -154,62 +201,66 @@ __device__ __forceinline__ bool writers_agree(bool ok) {
 // 148 SMs, and three left over); a run's short tile comes first, where the ring is filling anyway.  Several tiles of
 // rows: whole tiles, those of the same vocabulary rows next to each other, so that W comes from HBM once and from
 // L2 after that.
+template <bool PAIR>
 struct HeadTiles {
-    int unit, unit_end, t, n_tiles, row_tiles;
+    int unit, unit_end, t, n_tiles, row_tiles, rank;
     __device__ explicit HeadTiles(const HeadArgs& a) {
+        const int index = PAIR ? blockIdx.x / 2 : blockIdx.x, count = PAIR ? gridDim.x / 2 : gridDim.x;
+        rank = PAIR ? blockIdx.x & 1 : 0;
         row_tiles = a.row_tiles;
-        const long long units = (a.vocab + UNIT - 1) / UNIT;
-        unit = (int)(units * blockIdx.x / gridDim.x);
-        unit_end = (int)(units * (blockIdx.x + 1) / gridDim.x);
-        t = blockIdx.x;
+        const long long units = (a.vocab + UNIT * CTAS - 1) / (UNIT * CTAS);
+        unit = (int)(units * index / count);
+        unit_end = (int)(units * (index + 1) / count);
+        t = index;
         n_tiles = a.v_tiles * a.row_tiles;
     }
-    // false: no more
+    // This CTA's part of the next tile; false: no more.
     __device__ bool next(int* v0, int* v_rows, int* row_tile) {
         if (row_tiles == 1) {
             if (unit >= unit_end) return false;
             const int odd = (unit_end - unit) % (VT / UNIT), n = odd ? odd : VT / UNIT;
-            *v0 = unit * UNIT;
             *v_rows = n * UNIT;
+            *v0 = unit * (UNIT * CTAS) + rank * *v_rows;
             *row_tile = 0;
             unit += n;
             return true;
         }
         if (t >= n_tiles) return false;
-        *v0 = t / row_tiles * VT;
+        *v0 = (t / row_tiles * CTAS + rank) * VT;
         *v_rows = VT;
         *row_tile = t % row_tiles;
-        t += gridDim.x;
+        t += PAIR ? gridDim.x / 2 : gridDim.x;
         return true;
     }
+    static constexpr int CTAS = PAIR ? 2 : 1;
 };
 
 // The adapters' steps of a tile, packed into stages as they come: up to the stage's room for B and for u.
+template <bool PAIR>
 struct HeadPacks {
     const HeadSlot* slots;
-    int at, end, chunk, chunks, most, room, row_bytes;
+    int at, end, chunk, chunks, room;
     __device__ HeadPacks(const HeadArgs& a, int row_tile) {
         slots = a.slots;
         at = a.tile_first[row_tile];
         end = a.tile_first[row_tile + 1];
         chunk = 0;
-        chunks = (a.rank + a.u_cols - 1) / a.u_cols;
-        row_bytes = a.u_cols * 4;
-        most = A_BYTES / (VT * a.u_cols * 2);
+        chunks = a.chunks;
         room = a.stage_bytes - A_BYTES;
     }
-    // The steps of the next stage; 0: no more.
+    // The steps of the next stage, and the bytes of u that this CTA holds of them; 0: no more.
     __device__ int next(HeadSlot slot[MAX_PACK], int chunk_of[MAX_PACK], int* u_bytes) {
         int n = 0;
         *u_bytes = 0;
 #pragma unroll
         for (int i = 0; i < MAX_PACK; i++) {
-            if (i < most && n == i && at < end) {
+            if (n == i && at < end) {
                 const HeadSlot s = slots[at];
-                if (*u_bytes + s.n * row_bytes <= room) {
+                const int bytes = s.n / (PAIR ? 2 : 1) * U_BYTES;
+                if (*u_bytes + bytes <= room) {
                     slot[i] = s;
                     chunk_of[i] = chunk;
-                    *u_bytes += s.n * row_bytes;
+                    *u_bytes += bytes;
                     n++;
                     if (++chunk == chunks) chunk = 0, at++;
                 }
@@ -239,6 +290,9 @@ __global__ void __launch_bounds__(HEAD_NT, 1) head_rows_kernel(const HeadArgs a,
     constexpr int ROUND = E4M3 ? ROUND_E4M3 : ROUND_BF16;
     constexpr int OUT_BYTES = OUT16 ? 2 : 4;
     using Out = typename OutType<OUT16>::type;
+    constexpr bool PAIR = GROUPS >= 4;
+    constexpr int CTAS = PAIR ? 2 : 1;
+    const bool lead = !PAIR || (blockIdx.x & 1) == 0;
     const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
     char* const ring = raw + (base - smem_u32(raw));
     const uint32_t zeros = base + (uint32_t)(a.stages * a.stage_bytes);
@@ -259,21 +313,27 @@ __global__ void __launch_bounds__(HEAD_NT, 1) head_rows_kernel(const HeadArgs a,
         }
         for (int i = 0; i < 2; i++) {
             mbar_init(&ctl.acc_full[i], 1);
-            mbar_init(&ctl.acc_empty[i], WRITERS / 32);
+            mbar_init(&ctl.acc_empty[i], WRITERS / 32 * CTAS);
         }
         mbar_init(&ctl.drain, 1);
         ctl.abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    __syncwarp();
     if (warp == WRITERS / 32 + 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&ctl.tmem)) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        if (PAIR) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&ctl.tmem)) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&ctl.tmem)) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        }
         tmem_fence_before();
     }
-    __syncthreads();
+    sync_all<PAIR>();
     tmem_fence_after();
     const uint32_t tmem = ctl.tmem;
-    HeadTiles tiles(a);
+    HeadTiles<PAIR> tiles(a);
     int v0, v_rows, row_tile;
     // what the kernels in front wrote may be read from here on (each thread asks once, where it first needs it)
     bool behind = false;
@@ -293,17 +353,21 @@ __global__ void __launch_bounds__(HEAD_NT, 1) head_rows_kernel(const HeadArgs a,
                 fill++;
                 if (++stage == a.stages) stage = 0, phase ^= 1;
             };
+            // the even CTA of a pair awaits the bytes of both; a barrier counts them in any order
+            auto expect = [&](int bytes) { if (lead) mbar_expect(&ctl.full[stage], (uint32_t)bytes * CTAS); };
+            const int x_rows = a.tile_cols / CTAS, half = PAIR ? blockIdx.x & 1 : 0;
             auto load_w = [&](int s) {
-                const uint32_t dst = base + (uint32_t)(stage * a.stage_bytes);
-                mbar_expect(&ctl.full[stage], (uint32_t)((v_rows + a.tile_cols) * STEP_BYTES));
+                const uint32_t dst = base + (uint32_t)(stage * a.stage_bytes), bar = lead_bar<PAIR>(&ctl.full[stage]);
+                expect((v_rows + x_rows) * STEP_BYTES);
                 if (v_rows == VT) {
-                    tma_2d(dst, &maps.w, s * STEP_COLS, v0, &ctl.full[stage]);
+                    tma_2d<PAIR>(dst, &maps.w, s * STEP_COLS, v0, bar);
                 } else {
-                    for (int i = 0; i < v_rows; i += UNIT) tma_2d(dst + i * STEP_BYTES, &maps.w16, s * STEP_COLS, v0 + i, &ctl.full[stage]);
+                    for (int i = 0; i < v_rows; i += UNIT) tma_2d<PAIR>(dst + i * STEP_BYTES, &maps.w16, s * STEP_COLS, v0 + i, bar);
                 }
             };
             auto load_x = [&](int s, int st) {
-                tma_2d(base + (uint32_t)(st * a.stage_bytes + A_BYTES), &maps.x, s * STEP_COLS, row_tile * a.tile_cols, &ctl.full[st]);
+                tma_2d<PAIR>(base + (uint32_t)(st * a.stage_bytes + A_BYTES), &maps.x, s * STEP_COLS, row_tile * a.tile_cols + half * x_rows,
+                             lead_bar<PAIR>(&ctl.full[st]));
             };
             while (ok && tiles.next(&v0, &v_rows, &row_tile)) {
                 int s = 0;
@@ -329,28 +393,29 @@ __global__ void __launch_bounds__(HEAD_NT, 1) head_rows_kernel(const HeadArgs a,
                     wait_for_front();
                     asm volatile("fence.proxy.async.global;" ::: "memory");
                 }
-                HeadPacks packs(a, row_tile);
+                HeadPacks<PAIR> packs(a, row_tile);
                 HeadSlot slot[MAX_PACK];
                 int chunk[MAX_PACK], u_bytes;
                 while (const int n = packs.next(slot, chunk, &u_bytes)) {
                     if (!take()) break;
-                    const uint32_t dst = base + (uint32_t)(stage * a.stage_bytes);
-                    uint64_t* bar = &ctl.full[stage];
-                    mbar_expect(bar, (uint32_t)(n * v_rows * a.u_cols * 2 + u_bytes));
+                    const uint32_t dst = base + (uint32_t)(stage * a.stage_bytes), bar = lead_bar<PAIR>(&ctl.full[stage]);
+                    expect(n * v_rows * U_RANKS * 2 + u_bytes);
                     uint32_t u_dst = dst + A_BYTES;
 #pragma unroll
                     for (int i = 0; i < MAX_PACK; i++) {
                         if (i >= n) continue;
-                        const uint32_t b_dst = dst + (uint32_t)(i * VT * a.u_cols * 2);
+                        const uint32_t b_dst = dst + (uint32_t)(i * B_BYTES);
+                        const int row = chunk[i] * a.b_rows + v0 / 4;  // four vocabulary rows to 128 bytes
                         if (v_rows == VT) {
-                            tma_3d(b_dst, &maps.b, chunk[i] * a.u_cols, v0, slot[i].adapter, bar);
+                            tma_3d<PAIR>(b_dst, &maps.b, 0, row, slot[i].adapter, bar);
                         } else {
-                            for (int r = 0; r < v_rows; r += UNIT)
-                                tma_3d(b_dst + r * a.u_cols * 2, &maps.b16, chunk[i] * a.u_cols, v0 + r, slot[i].adapter, bar);
+                            for (int r = 0; r < v_rows / 4; r += UNIT / 4)
+                                tma_3d<PAIR>(b_dst + r * 128, &maps.b16, 0, row + r, slot[i].adapter, bar);
                         }
-                        for (int r = 0; r < slot[i].n; r += a.u_box)
-                            tma_2d(u_dst + r * a.u_cols * 4, &maps.u, 0, chunk[i] * a.u_rows + slot[i].u_row + r, bar);
-                        u_dst += (uint32_t)(slot[i].n * a.u_cols * 4);
+                        const int u_n = slot[i].n / CTAS, u_row = chunk[i] * a.u_rows + slot[i].u_row + half * u_n;
+                        for (int r = 0; r < u_n; r += a.u_box)  // two rows of u to 128 bytes
+                            tma_2d<PAIR>(u_dst + r * U_BYTES, &maps.u, 0, (u_row + r) / 2, bar);
+                        u_dst += (uint32_t)(u_n * U_BYTES);
                     }
                     advance();
                 }
@@ -370,7 +435,7 @@ __global__ void __launch_bounds__(HEAD_NT, 1) head_rows_kernel(const HeadArgs a,
         }
         __syncwarp();
     } else if (warp == WRITERS / 32 + 1) {
-        if (lane == 0) {
+        if (lane == 0 && lead) {
             int stage = 0, round = 0;
             uint32_t phase = 0;
             bool ok = true;
@@ -380,7 +445,7 @@ __global__ void __launch_bounds__(HEAD_NT, 1) head_rows_kernel(const HeadArgs a,
                 return ok;
             };
             auto advance = [&]() {
-                mma_commit(&ctl.empty[stage]);
+                mma_commit<PAIR>(&ctl.empty[stage]);
                 if (++stage == a.stages) stage = 0, phase ^= 1;
             };
             uint32_t acc = 0;
@@ -390,10 +455,9 @@ __global__ void __launch_bounds__(HEAD_NT, 1) head_rows_kernel(const HeadArgs a,
                 acc = tmem + (uint32_t)(round & 1) * MAX_COLS;
                 return ok;
             };
-            auto end_round = [&]() { mma_commit(&ctl.acc_full[round++ & 1]); };
-            const uint32_t shape = E4M3 ? shape_e4m3(a.tile_cols) : shape_bf16(a.tile_cols);
-            const uint64_t wide = operand_format(128), zero = operand(operand_format(32), zeros);
-            const uint64_t b_format = operand_format(a.u_cols * 2), u_format = operand_format(a.u_cols * 4);
+            auto end_round = [&]() { mma_commit<PAIR>(&ctl.acc_full[round++ & 1]); };
+            const uint32_t shape = E4M3 ? shape_e4m3<PAIR>(a.tile_cols) : shape_bf16<PAIR>(a.tile_cols);
+            const uint64_t zero = operand(blocks(U_RANKS * 16), zeros);
             while (ok && tiles.next(&v0, &v_rows, &row_tile)) {
                 for (int s = 0; s < a.w_steps; s++) {
                     const bool first = s % ROUND == 0;
@@ -402,9 +466,7 @@ __global__ void __launch_bounds__(HEAD_NT, 1) head_rows_kernel(const HeadArgs a,
                     const uint32_t src = base + (uint32_t)(stage * a.stage_bytes);
 #pragma unroll
                     for (int k = 0; k < STEP_BYTES; k += 32) {
-                        const uint64_t wd = operand(wide, src + k), xd = operand(wide, src + A_BYTES + k);
-                        if (E4M3) mma_e4m3(acc, wd, xd, shape, !first || k > 0);
-                        else mma_bf16(acc, wd, xd, shape, !first || k > 0);
+                        mma<PAIR, E4M3>(acc, operand(SWIZZLED_ROWS, src + k), operand(SWIZZLED_ROWS, src + A_BYTES + k), shape, !first || k > 0);
                     }
                     advance();
                     if (s % ROUND == ROUND - 1 || s == a.w_steps - 1) {
@@ -413,12 +475,12 @@ __global__ void __launch_bounds__(HEAD_NT, 1) head_rows_kernel(const HeadArgs a,
                 }
                 if (!ok || !a.slots_on) continue;
                 wait_for_front();
-                HeadPacks packs(a, row_tile);
+                HeadPacks<PAIR> packs(a, row_tile);
                 if (own_round) {
                     if (packs.at == packs.end) continue;
                     if (!begin_round()) break;
                     // the slots' windows may cover a tile in part only: zero times zero first
-                    mma_bf16(acc, zero, zero, shape_bf16(a.tile_cols), false);
+                    mma<PAIR, false>(acc, zero, zero, shape_bf16<PAIR>(a.tile_cols), false);
                 }
                 HeadSlot slot[MAX_PACK];
                 int chunk[MAX_PACK], u_bytes;
@@ -429,21 +491,18 @@ __global__ void __launch_bounds__(HEAD_NT, 1) head_rows_kernel(const HeadArgs a,
 #pragma unroll
                     for (int i = 0; i < MAX_PACK; i++) {
                         if (i >= n) continue;
-                        const uint32_t d = acc + (uint32_t)slot[i].col, n_shape = shape_bf16(slot[i].n);
-                        const uint32_t b_src = src + (uint32_t)(i * VT * a.u_cols * 2);
-                        for (int k = 0; k < a.u_cols && chunk[i] * a.u_cols + k < a.rank; k += 16) {
-                            const uint64_t bd = operand(b_format, b_src + k * 2);
-                            mma_bf16(d, bd, operand(u_format, u_src + k * 2), n_shape, true);
-                            mma_bf16(d, bd, operand(u_format, u_src + (a.u_cols + k) * 2), n_shape, true);
-                        }
-                        u_src += (uint32_t)(slot[i].n * a.u_cols * 4);
+                        const uint32_t d = acc + (uint32_t)slot[i].col, n_shape = shape_bf16<PAIR>(slot[i].n);
+                        const uint64_t bd = operand(blocks(U_RANKS * 16), src + (uint32_t)(i * B_BYTES));
+                        mma<PAIR, false>(d, bd, operand(blocks(U_BYTES * 8), u_src), n_shape, true);
+                        mma<PAIR, false>(d, bd, operand(blocks(U_BYTES * 8), u_src + 256), n_shape, true);
+                        u_src += (uint32_t)(slot[i].n / CTAS * U_BYTES);
                     }
                     advance();
                 }
                 if (ok) end_round();
             }
             if (!ok) {  // what was issued ends before tensor memory is given back
-                mma_commit(&ctl.drain);
+                mma_commit<PAIR>(&ctl.drain);
                 mbar_wait(&ctl.drain, 0, 100000000ull);
             }
         }
@@ -517,7 +576,7 @@ __global__ void __launch_bounds__(HEAD_NT, 1) head_rows_kernel(const HeadArgs a,
                     tmem_fence_before();
                 }
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&ctl.acc_empty[round & 1]);
+                if (lane == 0) lead_arrive<PAIR>(&ctl.acc_empty[round & 1]);
             }
             if (ok && mine) {
                 char* to = static_cast<char*>(a.out) + (long long)v * OUT_BYTES;
@@ -535,9 +594,12 @@ __global__ void __launch_bounds__(HEAD_NT, 1) head_rows_kernel(const HeadArgs a,
             ok = writers_agree(ok);  // the tables are free, and the warps go on together or not at all
         }
     }
-    __syncthreads();
+    sync_all<PAIR>();  // a pair's products read both CTAs' shared memory, and their ends arrive in both
     if (threadIdx.x == 0 && ctl.abort && a.status) atomicOr(a.status, MANTLE_SAMPLE_STATUS_TIMEOUT);
-    if (warp == WRITERS / 32 + 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    if (warp == WRITERS / 32 + 1) {
+        if (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+        else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    }
 }
 
 }  // namespace

@@ -178,6 +178,7 @@ class Adapters:
     a     [n, rank, hidden] bfloat16     b     [n, vocab, rank] bfloat16, both contiguous
     gain  optional [n] float32 (alpha / rank, usually)
     rank is a multiple of 8; adapters of smaller rank are padded with zeros.  Everything in a and b is finite.
+    b is copied into the layout the projection reads (on the current stream, once); a and gain are kept as they are.
     """
 
     def __init__(self, a, b, gain=None):
@@ -188,8 +189,37 @@ class Adapters:
             raise ValueError("a is [n, rank, hidden] and b [n, vocab, rank], on one device")
         if gain is not None:
             _vector(gain, "gain", a.shape[0], (torch.float32,), a.device)
-        self.a, self.b, self.gain = a, b, gain
-        self.n, self.rank = a.shape[0], a.shape[1]
+        self.lib = native.load()
+        self.a, self.gain, self.device = a, gain, a.device
+        self.n, self.rank, self.hidden, self.vocab = a.shape[0], a.shape[1], a.shape[2], b.shape[1]
+        n = C.c_size_t(0)
+        _check(self.lib, self.lib.mantleCudaAdapterPackBytes(1, self.vocab, self.rank, C.byref(n)), "mantleCudaAdapterPackBytes")
+        self._one = n.value
+        self.packed = torch.empty(self.n * self._one, dtype=torch.uint8, device=a.device)
+        self._pack(b, 0, self.n)
+
+    def _pack(self, b, first, n):
+        with torch.cuda.device(self.device):
+            rc = self.lib.mantleCudaAdapterPack(b.data_ptr(), n, self.vocab, self.rank, self.packed.data_ptr() + first * self._one,
+                                                torch.cuda.current_stream().cuda_stream)
+        _check(self.lib, rc, "mantleCudaAdapterPack")
+
+    def replace(self, i, a, b, gain=None):
+        """Puts another adapter, a [rank, hidden] and b [vocab, rank], in the place of adapter i, on the current
+        stream of the table's device.  gain is a number, given exactly when the table has gains."""
+        if not 0 <= i < self.n:
+            raise ValueError("no adapter %d in a table of %d" % (i, self.n))
+        if (gain is None) != (self.gain is None):
+            raise ValueError("gain is needed exactly when the table has gains")
+        for t, name, shape in ((a, "a", (self.rank, self.hidden)), (b, "b", (self.vocab, self.rank))):
+            if t.device != self.device or tuple(t.shape) != shape or t.dtype != torch.bfloat16 or not t.is_contiguous():
+                raise ValueError("%s must be a contiguous %s bfloat16 tensor on %s" % (name, shape, self.device))
+        if b.data_ptr() % 16:
+            raise ValueError("b must start on 16 bytes")
+        self.a[i].copy_(a)
+        if gain is not None:
+            self.gain[i].fill_(gain)
+        self._pack(b, i, 1)
 
 
 class HeadPlan(_Plan):
@@ -246,11 +276,11 @@ class HeadPlan(_Plan):
         if (adapters is None) != (adapter_ids is None):
             raise ValueError("adapters and adapter_ids go together")
         if adapters is not None:
-            if adapters.a.device != dev or adapters.a.shape[2] != k or adapters.b.shape[1] != vocab:
+            if adapters.device != dev or adapters.hidden != k or adapters.vocab != vocab:
                 raise ValueError("the adapters are for another projection: [%d, %d] on %s"
-                                 % (adapters.b.shape[1], adapters.a.shape[2], adapters.a.device))
+                                 % (adapters.vocab, adapters.hidden, adapters.device))
             _vector(adapter_ids, "adapter_ids", rows, (torch.int32,), dev)
-            b.adapter_a, b.adapter_b = adapters.a.data_ptr(), adapters.b.data_ptr()
+            b.adapter_a, b.adapter_b = adapters.a.data_ptr(), adapters.packed.data_ptr()
             b.adapter_gain = None if adapters.gain is None else adapters.gain.data_ptr()
             b.adapter_ids, b.n_adapters, b.rank = adapter_ids.data_ptr(), adapters.n, adapters.rank
         if out is None:
@@ -258,7 +288,7 @@ class HeadPlan(_Plan):
         b.out_dtype, b.out_stride = _rows(out, "out", (out_dtype,), dev, (rows, vocab))
         b.out, b.vocab = out.data_ptr(), vocab
         reads = [hidden, weight, base, hidden_scales, weight_scales, adapter_ids]
-        reads += [adapters.a, adapters.b, adapters.gain] if adapters is not None else []
+        reads += [adapters.a, adapters.packed, adapters.gain] if adapters is not None else []
         for t in reads:
             if t is not None and _overlap(out, t) and not (t is base and _same(out, base)):
                 raise ValueError("out overlaps an input")

@@ -217,6 +217,8 @@ BATCH_EXPORTS = {
 # include/mantle_head.h
 HEAD_EXPORTS = {
     "mantleCudaNormRows": (C.c_int, [C.POINTER(NormBatch), C.c_void_p]),
+    "mantleCudaAdapterPackBytes": (C.c_int, [C.c_int, C.c_int, C.c_int, C.POINTER(C.c_size_t)]),
+    "mantleCudaAdapterPack": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p]),
     "mantleCudaHeadRows": (C.c_int, [C.POINTER(HeadBatch), C.c_void_p, C.c_size_t, C.c_void_p]),
     "mantleCudaHeadWorkspaceBytes": (C.c_int, [C.POINTER(HeadBatch), C.POINTER(C.c_size_t)]),
     "mantleCudaHeadLaunches": (C.c_int, [C.POINTER(HeadBatch), C.POINTER(C.c_int)]),

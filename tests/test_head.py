@@ -85,7 +85,7 @@ def test_norm_refuses(change):
     dict(hidden_stride=63), dict(out_stride=99), dict(weight_stride=56), dict(weight_stride=68), dict(weight=0x2008), dict(weight_stride=1 << 37),
     dict(hidden_rows=0x1001), dict(out=0x3002), dict(status=0x9001), dict(n_adapters=-1), dict(ADAPTERS, n_adapters=4097),
     dict(ADAPTERS, adapter_a=0), dict(ADAPTERS, adapter_b=0), dict(ADAPTERS, adapter_ids=0), dict(ADAPTERS, adapter_ids=0x30002),
-    dict(ADAPTERS, rank=0), dict(ADAPTERS, rank=12), dict(ADAPTERS, rank=264), dict(ADAPTERS, adapter_a=0x10008), dict(ADAPTERS, adapter_b=0x20008),
+    dict(ADAPTERS, rank=0), dict(ADAPTERS, rank=12), dict(ADAPTERS, rank=264), dict(ADAPTERS, adapter_a=0x10008), dict(ADAPTERS, adapter_b=0x20010),
     dict(ADAPTERS, adapter_gain=0x9001),
 ])
 def test_head_refuses(change):
