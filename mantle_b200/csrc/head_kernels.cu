@@ -149,9 +149,7 @@ HeadLayout head_layout(const MantleHeadBatch* b) {
     l.grid = (int)std::min<long long>(device_info().sms / ctas, work) * ctas;
     const bool own_round = l.adapters && (l.eight || !weight);
     const size_t fixed = 1024 + sizeof(HeadCtl) + (own_round ? ZERO_BYTES : 0);
-    // Adapters on the whole tile: room for four windows of u, as far as that is no more than W's share of the stage.
-    const int x_bytes = l.tile_cols / ctas * STEP_BYTES;
-    l.stage_bytes = A_BYTES + (l.adapters && !l.sorted ? std::max(x_bytes, std::min(2 * x_bytes, A_BYTES)) : x_bytes);
+    l.stage_bytes = A_BYTES + l.tile_cols / ctas * STEP_BYTES;
     l.stages = (int)std::min<size_t>(MAX_STAGES, ((size_t)232448 - fixed) / (size_t)l.stage_bytes);
     l.smem = fixed + (size_t)l.stages * (size_t)l.stage_bytes;
 
@@ -255,7 +253,7 @@ int launch_head_as(const HeadArgs& a, const HeadMaps& maps, const HeadLayout& l,
 template <bool E4M3, bool OUT16>
 int launch_head(const HeadArgs& a, const HeadMaps& maps, const HeadLayout& l, cudaStream_t stream) {
     if (l.tile_cols <= 32) return launch_head_as<E4M3, OUT16, 1>(a, maps, l, stream);
-    if (!l.pair) return launch_head_as<E4M3, OUT16, 2>(a, maps, l, stream);
+    if (l.tile_cols <= 64) return launch_head_as<E4M3, OUT16, 2>(a, maps, l, stream);
     if (l.tile_cols <= 128) return launch_head_as<E4M3, OUT16, 4>(a, maps, l, stream);
     return launch_head_as<E4M3, OUT16, 8>(a, maps, l, stream);
 }
@@ -356,6 +354,8 @@ extern "C" int mantleCudaHeadRows(const MantleHeadBatch* b, void* workspace, siz
     a.b_rows = padded / 4;
     a.stages = l.stages;
     a.stage_bytes = l.stage_bytes;
+    a.pack_bytes = B_BYTES + l.tile_cols / (l.pair ? 2 : 1) * U_BYTES;
+    a.pack = l.stage_bytes / a.pack_bytes;
     a.x_scales = b->hidden_scales;
     a.w_scales = b->weight_scales;
     a.base = b->base;
@@ -402,15 +402,14 @@ extern "C" int mantleCudaHeadRows(const MantleHeadBatch* b, void* workspace, siz
     bool ok = true;
     const int x_rows = l.tile_cols / (l.pair ? 2 : 1);
     if (b->weight) {
-        ok = ok && encode_rows(&maps.w, b->weight, l.eight, b->vocab, b->hidden, b->weight_stride * e, VT);
-        ok = ok && encode_rows(&maps.w16, b->weight, l.eight, b->vocab, b->hidden, b->weight_stride * e, UNIT);
+        for (int m = 0; m < 4; m++)
+            ok = ok && encode_rows(&maps.w[m], b->weight, l.eight, b->vocab, b->hidden, b->weight_stride * e, VT >> m);
         ok = ok && (p.xs ? encode_rows(&maps.x, p.xs, l.eight, b->rows, b->hidden, b->hidden * e, x_rows)
                          : encode_rows(&maps.x, b->hidden_rows, l.eight, b->rows, b->hidden, b->hidden_stride * e, x_rows));
     }
     if (l.adapters) {
         const long long per_adapter = (long long)l.chunks * a.b_rows;
-        ok = ok && encode_plain(&maps.b, b->adapter_b, per_adapter, b->n_adapters, VT / 4);
-        ok = ok && encode_plain(&maps.b16, b->adapter_b, per_adapter, b->n_adapters, UNIT / 4);
+        for (int m = 0; m < 4; m++) ok = ok && encode_plain(&maps.b[m], b->adapter_b, per_adapter, b->n_adapters, (VT >> m) / 4);
         ok = ok && encode_plain(&maps.u, p.u, (long long)l.chunks * l.u_rows / 2, 0, a.u_box / 2);
     }
     if (!ok) return refuse("head: the driver refused a tensor map");
@@ -421,7 +420,7 @@ extern "C" int mantleCudaHeadRows(const MantleHeadBatch* b, void* workspace, siz
         if (rc) return rc;
     }
     if (l.adapters || l.copied) {
-        const dim3 grid((unsigned)(p.units + p.copy_ctas), (unsigned)(l.adapters ? b->rank / 8 : 1));
+        const dim3 grid((unsigned)(p.units + p.copy_ctas), (unsigned)std::max(1, l.chunks));
         rc = l.sorted ? launch<HeadPrep>(head_shrink_kernel, grid, SHRINK_NT, 0, stream, true, false, p)
                       : launch<HeadPrep>(head_shrink_here_kernel, grid, SHRINK_NT, 0, stream, false, false, p);
         if (rc) return rc;

@@ -216,43 +216,57 @@ __device__ __forceinline__ void copy_rows(const HeadPrep& p, int first, int step
     }
 }
 
-// Eight ranks (from j0) of sixteen rows' products with one adapter's A: rows[i] is the row of x of place i, -1 none.
+// One chunk of ranks (from j0) of 32 rows' products with one adapter's A: rows[i] is the row of x of place i, -1 none.
 // The warps share out the columns of x and add their sums up in shared memory.  The order of the columns within
 // a step is free in a dot product, so each lane takes eight neighbours of its row, one 16-byte load, as two
-// steps' operands.  On return thread i * 8 + j of the first 128 holds place i, rank j0 + j.
-__device__ __forceinline__ float shrink16(const HeadPrep& p, int adapter, int j0, const int* rows, float (*sums)[16][8]) {
+// steps' operands.  On return thread i * 16 + j holds place i, rank j0 + j.
+typedef float ShrinkSums[SHRINK_WARPS][32][U_RANKS];
+__device__ __forceinline__ float shrink32(const HeadPrep& p, int adapter, int j0, const int* rows, ShrinkSums& sums) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
     const int esz = p.e4m3 ? 1 : 2;
-    const char* row[2];
+    const char* row[4];
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
+    for (int i = 0; i < 4; i++) {
         const int r = rows[g + 8 * i];
         row[i] = r >= 0 ? static_cast<const char*>(p.x) + (long long)r * p.x_stride * esz : nullptr;
     }
     const bf16_raw* arow = p.a + ((long long)adapter * p.rank + j0 + g) * p.hidden;
-    float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    const bool both = j0 + 8 < p.rank;  // (the rank may end after eight)
+    float d[2][2][4] = {};
     const uint4 none = make_uint4(0, 0, 0, 0);
-#pragma unroll 4
+#pragma unroll 2
     for (int k = warp * 32 + q * 8; k < p.hidden + q * 8; k += SHRINK_WARPS * 32) {  // the same count for a warp's lanes
         const bool in = k < p.hidden;
-        const uint4 b = in ? *reinterpret_cast<const uint4*>(arow + k) : none;
-        const uint4 x0 = in && row[0] ? x_eight(p, row[0], k) : none;
-        const uint4 x1 = in && row[1] ? x_eight(p, row[1], k) : none;
-        mma_16x8x16(d, x0.x, x1.x, x0.y, x1.y, b.x, b.y);
-        mma_16x8x16(d, x0.z, x1.z, x0.w, x1.w, b.z, b.w);
-    }
-    sums[warp][g][q * 2] = d[0], sums[warp][g][q * 2 + 1] = d[1];
-    sums[warp][g + 8][q * 2] = d[2], sums[warp][g + 8][q * 2 + 1] = d[3];
-    __syncthreads();
-    float v = 0.0f;
-    if (threadIdx.x < 128) {
-        const int i = threadIdx.x >> 3, j = threadIdx.x & 7, r = rows[i];
-        if (r >= 0) {
+        uint4 x[4], w[2];
 #pragma unroll
-            for (int w = 0; w < SHRINK_WARPS; w++) v += sums[w][i][j];
-            if (p.gain) v *= p.gain[adapter];
-            if (p.e4m3) v *= p.x_scales[r];
+        for (int i = 0; i < 4; i++) x[i] = in && row[i] ? x_eight(p, row[i], k) : none;
+        w[0] = in ? *reinterpret_cast<const uint4*>(arow + k) : none;
+        w[1] = in && both ? *reinterpret_cast<const uint4*>(arow + 8ll * p.hidden + k) : none;
+#pragma unroll
+        for (int m = 0; m < 2; m++) {
+#pragma unroll
+            for (int n = 0; n < 2; n++) {
+                mma_16x8x16(d[m][n], x[2 * m].x, x[2 * m + 1].x, x[2 * m].y, x[2 * m + 1].y, w[n].x, w[n].y);
+                mma_16x8x16(d[m][n], x[2 * m].z, x[2 * m + 1].z, x[2 * m].w, x[2 * m + 1].w, w[n].z, w[n].w);
+            }
         }
+    }
+#pragma unroll
+    for (int m = 0; m < 2; m++) {
+#pragma unroll
+        for (int n = 0; n < 2; n++) {
+            sums[warp][m * 16 + g][n * 8 + q * 2] = d[m][n][0], sums[warp][m * 16 + g][n * 8 + q * 2 + 1] = d[m][n][1];
+            sums[warp][m * 16 + g + 8][n * 8 + q * 2] = d[m][n][2], sums[warp][m * 16 + g + 8][n * 8 + q * 2 + 1] = d[m][n][3];
+        }
+    }
+    __syncthreads();
+    const int i = threadIdx.x >> 4, j = threadIdx.x & 15, r = rows[i];
+    float v = 0.0f;
+    if (r >= 0) {
+#pragma unroll
+        for (int w = 0; w < SHRINK_WARPS; w++) v += sums[w][i][j];
+        if (p.gain) v *= p.gain[adapter];
+        if (p.e4m3) v *= p.x_scales[r];
     }
     return v;
 }
@@ -265,8 +279,7 @@ __device__ __forceinline__ bf16_raw* u_at(const HeadPrep& p, int rank_at, int u_
            (rank_at % U_RANKS / 8) * 64 + (u_row & 7) * 8 + rank_at % 8;
 }
 
-// v in two bfloat16: 16 bits of mantissa (an infinity or NaN stays in the leading part alone).  Where the rank ends
-// inside a chunk, the thread of its last eight also writes the zeros behind them.
+// v in two bfloat16: 16 bits of mantissa (an infinity or NaN stays in the leading part alone).
 __device__ __forceinline__ void store_u(const HeadPrep& p, int rank_at, int u_row, float v) {
     const uint32_t hi = pack_bf16(v, 0.0f) & 0xffffu;
     const float rest = v - __uint_as_float(hi << 16);
@@ -274,15 +287,11 @@ __device__ __forceinline__ void store_u(const HeadPrep& p, int rank_at, int u_ro
     bf16_raw* u = u_at(p, rank_at, u_row);
     u[0] = (bf16_raw)hi;
     u[128] = (bf16_raw)lo;
-    if (rank_at + 8 >= p.rank && p.rank % U_RANKS) {
-        u[64] = 0;
-        u[192] = 0;
-    }
 }
 
-// Sorted form.  CTAs [0, units) x [0, rank / 8): eight ranks of one box.  CTAs from `units` on: the copy of x.
+// Sorted form.  CTAs [0, units) x [0, chunks): one chunk of ranks of one box.  CTAs from `units` on: the copy of x.
 __global__ void __launch_bounds__(SHRINK_NT) head_shrink_kernel(const HeadPrep p) {
-    __shared__ float sums[SHRINK_WARPS][16][8];
+    __shared__ ShrinkSums sums;
     __shared__ int rows[WINDOW];
     pdl_trigger();
     pdl_wait();
@@ -298,22 +307,18 @@ __global__ void __launch_bounds__(SHRINK_NT) head_shrink_kernel(const HeadPrep p
         rows[threadIdx.x] = at >= box.first && at < box.last ? p.perm[at] : -1;
     }
     __syncthreads();
-    const int j0 = blockIdx.y * 8, j = threadIdx.x & 7, i = threadIdx.x >> 3;
-    for (int r = 0; r < WINDOW; r += 16) {
-        const bool some = box.first < box.place + r + 16 && box.last > box.place + r;
-        const float v = some ? shrink16(p, box.adapter, j0, rows + r, sums) : 0.0f;
-        if (threadIdx.x < 128) store_u(p, j0 + j, (int)blockIdx.x * WINDOW + r + i, v);
-        __syncthreads();
-    }
+    const int j0 = blockIdx.y * U_RANKS;
+    const float v = shrink32(p, box.adapter, j0, rows, sums);
+    store_u(p, j0 + (int)(threadIdx.x & 15), (int)blockIdx.x * WINDOW + (int)(threadIdx.x >> 4), v);
 }
 
-// Form for up to HERE_ROWS rows.  CTAs [0, units) x [0, rank / 8): eight ranks of the rows of one adapter -- the
+// Form for up to HERE_ROWS rows.  CTAs [0, units) x [0, chunks): a chunk of ranks of the rows of one adapter -- the
 // blockIdx.x-th of those in use, in the order of their first rows -- and zeros for the others.  CTAs from `units` on:
 // the copy of x, where its rows do not start on 16 bytes.
 __global__ void __launch_bounds__(SHRINK_NT) head_shrink_here_kernel(const HeadPrep p) {
-    __shared__ float sums[SHRINK_WARPS][16][8];
+    __shared__ ShrinkSums sums;
     __shared__ __align__(16) int ids[HERE_ROWS];
-    __shared__ int mine[HERE_ROWS + 16], first_of[HERE_ROWS];
+    __shared__ int mine[HERE_ROWS], first_of[HERE_ROWS];
     __shared__ int counts[2 * (HERE_ROWS / 32)];
     pdl_trigger();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -328,7 +333,6 @@ __global__ void __launch_bounds__(SHRINK_NT) head_shrink_here_kernel(const HeadP
         ids[tid] = id >= 0 && id < p.n_adapters ? id : -1;
         mine[tid] = -1;
     }
-    if (tid < 16) mine[HERE_ROWS + tid] = -1;
     __syncthreads();
     if (tid < HERE_ROWS) {
         const int id = ids[tid];
@@ -356,7 +360,7 @@ __global__ void __launch_bounds__(SHRINK_NT) head_shrink_here_kernel(const HeadP
         if (tid < 2) p.tile_first[tid] = tid ? in_use : 0;
     }
     if ((int)blockIdx.x >= in_use) return;
-    const int adapter = ids[first_of[blockIdx.x]], j0 = blockIdx.y * 8, u_row = (int)blockIdx.x * p.tile_cols;
+    const int adapter = ids[first_of[blockIdx.x]], j0 = blockIdx.y * U_RANKS, u_row = (int)blockIdx.x * p.tile_cols;
     if (tid < HERE_ROWS) {
         const bool use = ids[tid] == adapter;
         const uint32_t votes = __ballot_sync(0xffffffffu, use);
@@ -366,14 +370,14 @@ __global__ void __launch_bounds__(SHRINK_NT) head_shrink_here_kernel(const HeadP
         for (int w = 0; w < warp; w++) at += counts[HERE_ROWS / 32 + w];
         if (use) mine[at] = tid;
     }
-    for (int i = tid; i < p.tile_cols * 8; i += SHRINK_NT)
-        if (i / 8 >= HERE_ROWS || ids[i / 8] != adapter) store_u(p, j0 + i % 8, u_row + i / 8, 0.0f);
+    for (int i = tid; i < p.tile_cols * U_RANKS; i += SHRINK_NT)
+        if (ids[i / U_RANKS] != adapter) store_u(p, j0 + i % U_RANKS, u_row + i / U_RANKS, 0.0f);
     __syncthreads();
     int n = 0;
     for (int w = 0; w < HERE_ROWS / 32; w++) n += counts[HERE_ROWS / 32 + w];
-    for (int i = 0; i < n; i += 16) {
-        const float v = shrink16(p, adapter, j0, mine + i, sums);
-        if (tid < 128 && i + (tid >> 3) < n) store_u(p, j0 + (tid & 7), u_row + mine[i + (tid >> 3)], v);
+    for (int i = 0; i < n; i += 32) {
+        const float v = shrink32(p, adapter, j0, mine + i, sums);
+        if (i + (tid >> 4) < n) store_u(p, j0 + (tid & 15), u_row + mine[i + (tid >> 4)], v);
         __syncthreads();
     }
 }

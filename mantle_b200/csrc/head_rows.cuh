@@ -11,7 +11,10 @@
 // One CTA per SM, persistent over its tiles.  Warp 8 moves operands with TMA into a ring of stages (a stage: 128
 // rows of W, 128 bytes wide, and the same slice of x; or some adapters' B, 16 ranks wide, and their windows of u),
 // warp 9 issues tcgen05.mma from it, warps 0-7 read accumulators out of tensor memory, add them up in registers
-// and write the finished tile while the next one is computed.
+// and write the finished tile while the next one is computed.  Warp 10 works out, a lane each, what every step of the
+// tile's adapters copies and multiplies, ahead of warps 8 and 9, whose single threads then do little but issue:
+// instructions that are not a short loop cost such a thread ten to twenty cycles each (with slots read from L2 and
+// steps worked out by the issuing threads 16 adapters cost 64 rows 53 us, TODO us now).
 //
 // Pairs.  W comes from HBM once, but x from L2 for every 128 vocabulary rows: at 256 rows that is twice W's bytes,
 // and what L2 can hand out (about 10 TB/s) bounds the kernel long before HBM or the tensor cores do.  From 65 rows
@@ -42,14 +45,16 @@ constexpr int B_BYTES = VT * U_RANKS * 2;  // one adapter's B of one chunk and a
 constexpr int ROUND_BF16 = 8;      // steps of a round
 constexpr int ROUND_E4M3 = 64;
 constexpr int WRITERS = 256;       // threads that read accumulators and write results
-constexpr int HEAD_NT = WRITERS + 64;
+constexpr int HEAD_NT = WRITERS + 96;
 constexpr int ZERO_BYTES = VT * 32;
-constexpr int MAX_PACK = A_BYTES / B_BYTES;  // adapters' steps in one stage
+constexpr int SEGMENT = 96;        // adapters' steps that are worked out at a time; a multiple of 2, 3 and 4
 
-struct HeadCtl {
-    uint64_t full[MAX_STAGES], empty[MAX_STAGES], acc_full[2], acc_empty[2], drain;
+struct __align__(16) HeadCtl {
+    uint64_t full[MAX_STAGES], empty[MAX_STAGES], acc_full[2], acc_empty[2], steps_full[2], steps_empty[2], drain;
     uint32_t tmem;
     int abort;
+    int n_steps[2], more[2];  // of a segment, and whether the tile has another
+    int4 steps[2][SEGMENT];   // a step: row of its B in 128-byte rows, adapter, row of its u, first column and columns
     long long out_of[MAX_COLS], base_of[MAX_COLS];  // a column's row, as a distance in bytes
     float scale_of[MAX_COLS];
 };
@@ -58,6 +63,7 @@ struct HeadArgs {
     int rows, vocab, w_steps, tile_cols, row_tiles, v_tiles;
     int slots_on, sorted, copied;  // adapters; perm and x come from the kernel in front
     int chunks, u_rows, u_box;        // u_box: rows of u of one copy
+    int pack, pack_bytes;             // adapters' steps in one stage, and the room of each
     int b_rows;                       // 128-byte rows of one chunk of an adapter's B
     int stages, stage_bytes;
     const int* perm;
@@ -72,52 +78,67 @@ struct HeadArgs {
 };
 
 struct HeadMaps {
-    CUtensorMap w, w16, x, b, b16, u;  // (b, b16 and u: plain 128-byte rows)
+    CUtensorMap w[4], x, b[4], u;  // w and b: copies of 128, 64, 32 and 16 vocabulary rows; b and u: plain 128-byte rows
 };
 
 // ---- the instructions
+//
+// Warps 8 and 9 run as whole warps, all lanes with the same values, and only the instructions that act take a predicate
+// (`on`, true in one lane): the operands then live in the uniform registers that these instructions want.  As the
+// code of a single thread every stage's four products took 515 cycles to issue, whatever their size: that alone was
+// as long as W takes to come from HBM.
 
-__device__ __forceinline__ void mbar_expect(uint64_t* bar, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
-// The address of `bar` in the pair's even CTA (PAIR), or in this one.
+__device__ __forceinline__ void mbar_arrive_on(uint32_t bar, bool on) {
+    asm volatile("{.reg .pred q; setp.ne.b32 q, %1, 0; @q mbarrier.arrive.shared::cta.b64 _, [%0];}" ::"r"(bar), "r"((int)on) : "memory");
+}
+// Announces the bytes of a stage's copies; with `arrive` the announcement is complete.
+__device__ __forceinline__ void mbar_expect_on(uint32_t bar, uint32_t bytes, bool on) {
+    asm volatile("{.reg .pred q; setp.ne.b32 q, %2, 0; @q mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;}" ::"r"(bar), "r"(bytes), "r"((int)on) : "memory");
+}
+__device__ __forceinline__ void mbar_expect_more_on(uint32_t bar, uint32_t bytes, bool on) {
+    asm volatile("{.reg .pred q; setp.ne.b32 q, %2, 0; @q mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;}" ::"r"(bar), "r"(bytes), "r"((int)on) : "memory");
+}
+// The address of a barrier in the pair's even CTA (PAIR), or in this one.
 template <bool PAIR>
-__device__ __forceinline__ uint32_t lead_bar(uint64_t* bar) {
-    uint32_t at = smem_u32(bar);
-    if (PAIR) asm volatile("mapa.shared::cluster.u32 %0, %0, 0;" : "+r"(at));
-    return at;
+__device__ __forceinline__ uint32_t lead_bar(uint32_t bar) {
+    if (PAIR) asm volatile("mapa.shared::cluster.u32 %0, %0, 0;" : "+r"(bar));
+    return bar;
 }
 template <bool PAIR>
 __device__ __forceinline__ void lead_arrive(uint64_t* bar) {
-    if (PAIR) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(lead_bar<true>(bar)) : "memory");
-    else asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+    if (PAIR) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(lead_bar<true>(smem_u32(bar))) : "memory");
+    else mbar_arrive(bar);
 }
 // Copies to this CTA's shared memory that complete on a barrier of the pair's even CTA (bar: lead_bar's).
 template <bool PAIR>
-__device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+__device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar, bool on) {
     if (PAIR)
-        asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-                     ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
+        asm volatile("{.reg .pred q; setp.ne.b32 q, %5, 0; @q cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];}"
+                     ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar), "r"((int)on) : "memory");
     else
-        asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-                     ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
+        asm volatile("{.reg .pred q; setp.ne.b32 q, %5, 0; @q cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];}"
+                     ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar), "r"((int)on) : "memory");
 }
 template <bool PAIR>
-__device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+__device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar, bool on) {
     if (PAIR)
-        asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
-                     ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
+        asm volatile("{.reg .pred q; setp.ne.b32 q, %6, 0; @q cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];}"
+                     ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar), "r"((int)on) : "memory");
     else
-        asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
-                     ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
+        asm volatile("{.reg .pred q; setp.ne.b32 q, %6, 0; @q cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];}"
+                     ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar), "r"((int)on) : "memory");
 }
 
 // Shared-memory matrix descriptors of K-major operands.  W and x: rows of 128 bytes, swizzled, 1024 bytes from eight
 // rows to the next eight.  B and u: blocks of 8 rows by 16 bytes, 128 bytes from one block of a row to the next, and
 // `group` bytes from eight rows to the next eight.
-constexpr uint64_t SWIZZLED_ROWS = (uint64_t)1 << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
-__device__ constexpr uint64_t blocks(int group) { return (uint64_t)(128 >> 4) << 16 | (uint64_t)(group >> 4) << 32 | (uint64_t)1 << 46; }
-__device__ __forceinline__ uint64_t operand(uint64_t format, uint32_t addr) { return format | (uint64_t)((addr >> 4) & 0x3fff); }
+// (As two words: the low one holds the address and the distance of blocks, the high one all that does not change.)
+constexpr uint32_t SWIZZLED_ROWS_LO = 1u << 16, SWIZZLED_ROWS_HI = 1024u >> 4 | 1u << 14 | 2u << 29;
+constexpr uint32_t BLOCKS_LO = 128u >> 4 << 16, B_BLOCKS_HI = 256u >> 4 | 1u << 14, U_BLOCKS_HI = 512u >> 4 | 1u << 14;
+__device__ __forceinline__ uint32_t operand_lo(uint32_t format, uint32_t addr) { return format | ((addr >> 4) & 0x3fff); }
 // Instruction descriptor: float32 accumulator, 128 (a pair: 256) x n; bfloat16 operands, or e4m3.
 template <bool PAIR>
 __device__ __forceinline__ uint32_t shape_bf16(int n) {
@@ -128,10 +149,11 @@ __device__ __forceinline__ uint32_t shape_e4m3(int n) {
     return 1u << 4 | (uint32_t)(n >> 3) << 17 | (uint32_t)(VT * (PAIR ? 2 : 1) >> 4) << 24;
 }
 template <bool PAIR, bool E4M3>
-__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t shape, bool add) {
-#define MANTLE_MMA(GROUP, KIND)                                                                                          \
-    asm volatile("{.reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::" GROUP ".kind::" KIND " [%0], %1, %2, %3, p;}" \
-                 ::"r"(d), "l"(a), "l"(b), "r"(shape), "r"((int)add) : "memory")
+__device__ __forceinline__ void mma(uint32_t d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi, uint32_t shape, bool add, bool on) {
+#define MANTLE_MMA(GROUP, KIND)                                                                                                  \
+    asm volatile("{.reg .pred p, q; .reg .b64 a, b; setp.ne.b32 p, %6, 0; setp.ne.b32 q, %7, 0; mov.b64 a, {%1, %2}; mov.b64 b, {%3, %4}; " \
+                 "@q tcgen05.mma.cta_group::" GROUP ".kind::" KIND " [%0], a, b, %5, p;}"                                        \
+                 ::"r"(d), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(shape), "r"((int)add), "r"((int)on) : "memory")
     if (PAIR && E4M3) MANTLE_MMA("2", "f8f6f4");
     else if (PAIR) MANTLE_MMA("2", "f16");
     else if (E4M3) MANTLE_MMA("1", "f8f6f4");
@@ -140,12 +162,13 @@ __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t
 }
 // Arrives on `bar` -- of both CTAs of a pair -- when the products issued so far are done.
 template <bool PAIR>
-__device__ __forceinline__ void mma_commit(uint64_t* bar) {
+__device__ __forceinline__ void mma_commit(uint32_t bar, bool on) {
     if (PAIR)
-        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
-                     ::"r"(smem_u32(bar)), "h"((uint16_t)3) : "memory");
+        asm volatile("{.reg .pred q; setp.ne.b32 q, %2, 0; @q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;}"
+                     ::"r"(bar), "h"((uint16_t)3), "r"((int)on) : "memory");
     else
-        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+        asm volatile("{.reg .pred q; setp.ne.b32 q, %1, 0; @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];}"
+                     ::"r"(bar), "r"((int)on) : "memory");
 }
 // All threads of the CTA, or of the pair.
 template <bool PAIR>
@@ -182,6 +205,22 @@ __device__ __forceinline__ bool head_wait(uint64_t* bar, uint32_t parity, volati
             if (mbar_try_wait(bar, parity)) return true;
         if (*abort) return false;
         if (global_ns() - t0 > WAIT_LIMIT_NS) {
+            *abort = 1;
+            return false;
+        }
+    }
+}
+
+// The same for all lanes of a warp together.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    const uint64_t t0 = global_ns();
+    for (;;) {
+#pragma unroll 1
+        for (int i = 0; i < 8; i++)
+            if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+        if (__any_sync(0xffffffffu, *abort)) return false;
+        if (__any_sync(0xffffffffu, global_ns() - t0 > WAIT_LIMIT_NS)) {
             *abort = 1;
             return false;
         }
@@ -235,41 +274,6 @@ struct HeadTiles {
     static constexpr int CTAS = PAIR ? 2 : 1;
 };
 
-// The adapters' steps of a tile, packed into stages as they come: up to the stage's room for B and for u.
-template <bool PAIR>
-struct HeadPacks {
-    const HeadSlot* slots;
-    int at, end, chunk, chunks, room;
-    __device__ HeadPacks(const HeadArgs& a, int row_tile) {
-        slots = a.slots;
-        at = a.tile_first[row_tile];
-        end = a.tile_first[row_tile + 1];
-        chunk = 0;
-        chunks = a.chunks;
-        room = a.stage_bytes - A_BYTES;
-    }
-    // The steps of the next stage, and the bytes of u that this CTA holds of them; 0: no more.
-    __device__ int next(HeadSlot slot[MAX_PACK], int chunk_of[MAX_PACK], int* u_bytes) {
-        int n = 0;
-        *u_bytes = 0;
-#pragma unroll
-        for (int i = 0; i < MAX_PACK; i++) {
-            if (n == i && at < end) {
-                const HeadSlot s = slots[at];
-                const int bytes = s.n / (PAIR ? 2 : 1) * U_BYTES;
-                if (*u_bytes + bytes <= room) {
-                    slot[i] = s;
-                    chunk_of[i] = chunk;
-                    *u_bytes += bytes;
-                    n++;
-                    if (++chunk == chunks) chunk = 0, at++;
-                }
-            }
-        }
-        return n;
-    }
-};
-
 // ---- the kernel
 
 template <bool OUT16>
@@ -299,7 +303,7 @@ __global__ void __launch_bounds__(HEAD_NT, 1) head_rows_kernel(const HeadArgs a,
     // the adapters have a round of their own, or are the end of the projection's last one
     const bool own_round = a.slots_on && (E4M3 || a.w_steps == 0);
     HeadCtl& ctl = *reinterpret_cast<HeadCtl*>(ring + a.stages * a.stage_bytes + (own_round ? ZERO_BYTES : 0));
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
     if (own_round) {
         for (int i = threadIdx.x; i < ZERO_BYTES / 16; i += HEAD_NT)
@@ -314,6 +318,10 @@ __global__ void __launch_bounds__(HEAD_NT, 1) head_rows_kernel(const HeadArgs a,
         for (int i = 0; i < 2; i++) {
             mbar_init(&ctl.acc_full[i], 1);
             mbar_init(&ctl.acc_empty[i], WRITERS / 32 * CTAS);
+        }
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&ctl.steps_full[i], 1);
+            mbar_init(&ctl.steps_empty[i], lead ? 2 : 1);
         }
         mbar_init(&ctl.drain, 1);
         ctl.abort = 0;
@@ -341,169 +349,236 @@ __global__ void __launch_bounds__(HEAD_NT, 1) head_rows_kernel(const HeadArgs a,
         if (!behind) pdl_wait();
         behind = true;
     };
-
+    const uint32_t full0 = smem_u32(ctl.full), empty0 = smem_u32(ctl.empty);  // barriers of stage 0, 8 bytes each
     if (warp == WRITERS / 32) {
-        if (lane == 0) {
-            // fills of the ring, counted from the start; stage fill % stages
-            int fill = 0, stage = 0;
-            uint32_t phase = 1;  // of `empty`: the first round passes
-            bool ok = true;
-            auto take = [&]() { ok = head_wait(&ctl.empty[stage], phase, &ctl.abort); return ok; };
-            auto advance = [&]() {
-                fill++;
-                if (++stage == a.stages) stage = 0, phase ^= 1;
-            };
+        const bool on = lane == 0, on_lead = on && lead;
+        const int x_rows = a.tile_cols / CTAS, half = PAIR ? blockIdx.x & 1 : 0;
+        const uint32_t step_bytes = (uint32_t)a.stage_bytes;
+        int filled = 0, stage = 0, segment = 0;  // filled: stages in use so far
+        uint32_t phase = 1, dst = base;          // phase of `empty`: the first round passes
+        bool ok = true;
+        auto take = [&]() { return ok = warp_wait(empty0 + 8 * stage, phase, &ctl.abort); };
+        auto advance = [&]() {
+            filled = max(filled, ++stage);
+            dst += step_bytes;
+            if (stage == a.stages) stage = 0, phase ^= 1, dst = base;
+        };
+        auto load_w = [&](int s) {
+            const uint32_t bar = lead_bar<PAIR>(full0 + 8 * stage);
             // the even CTA of a pair awaits the bytes of both; a barrier counts them in any order
-            auto expect = [&](int bytes) { if (lead) mbar_expect(&ctl.full[stage], (uint32_t)bytes * CTAS); };
-            const int x_rows = a.tile_cols / CTAS, half = PAIR ? blockIdx.x & 1 : 0;
-            auto load_w = [&](int s) {
-                const uint32_t dst = base + (uint32_t)(stage * a.stage_bytes), bar = lead_bar<PAIR>(&ctl.full[stage]);
-                expect((v_rows + x_rows) * STEP_BYTES);
-                if (v_rows == VT) {
-                    tma_2d<PAIR>(dst, &maps.w, s * STEP_COLS, v0, bar);
-                } else {
-                    for (int i = 0; i < v_rows; i += UNIT) tma_2d<PAIR>(dst + i * STEP_BYTES, &maps.w16, s * STEP_COLS, v0 + i, bar);
+            mbar_expect_on(full0 + 8 * stage, (uint32_t)((v_rows + x_rows) * STEP_BYTES * CTAS), on_lead);
+            if (v_rows == VT) {
+                tma_2d<PAIR>(dst, &maps.w[0], s * STEP_COLS, v0, bar, on);
+                return;
+            }
+#pragma unroll 1
+            for (int m = 1, v = 0; m < 4; m++) {
+                if (v_rows & VT >> m) {
+                    tma_2d<PAIR>(dst + v * STEP_BYTES, &maps.w[m], s * STEP_COLS, v0 + v, bar, on);
+                    v += VT >> m;
                 }
-            };
-            auto load_x = [&](int s, int st) {
-                tma_2d<PAIR>(base + (uint32_t)(st * a.stage_bytes + A_BYTES), &maps.x, s * STEP_COLS, row_tile * a.tile_cols + half * x_rows,
-                             lead_bar<PAIR>(&ctl.full[st]));
-            };
-            while (ok && tiles.next(&v0, &v_rows, &row_tile)) {
-                int s = 0;
-                if (a.copied && !behind) {
-                    // W does not come from the kernels in front: the ring fills with it while they still run
-                    const int ahead = min(a.stages, a.w_steps);
-                    for (; s < ahead; s++) {
-                        load_w(s);
+            }
+        };
+        auto load_x = [&](int s, int st, uint32_t to) {
+            tma_2d<PAIR>(to + A_BYTES, &maps.x, s * STEP_COLS, row_tile * a.tile_cols + half * x_rows, lead_bar<PAIR>(full0 + 8 * st), on);
+        };
+        while (ok && tiles.next(&v0, &v_rows, &row_tile)) {
+            int s = 0;
+            if (a.copied && !behind) {
+                // W does not come from the kernels in front: the ring fills with it while they still run
+                const int ahead = min(a.stages, a.w_steps);
+                for (; s < ahead; s++) {
+                    load_w(s);
+                    advance();
+                }
+                wait_for_front();
+                asm volatile("fence.proxy.async.global;" ::: "memory");
+                for (int i = 0; i < ahead; i++) load_x(i, i, base + i * step_bytes);
+            }
+#pragma unroll 1
+            for (; s < a.w_steps; s++) {
+                if (!take()) break;
+                load_w(s);
+                load_x(s, stage, dst);
+                advance();
+            }
+            if (!ok || !a.slots_on) continue;
+            if (!behind) {
+                wait_for_front();
+                asm volatile("fence.proxy.async.global;" ::: "memory");
+            }
+            bool more = true;
+            for (; ok && more; segment++) {
+                const int table = segment & 1;
+                ok = warp_wait(smem_u32(&ctl.steps_full[table]), (segment >> 1) & 1, &ctl.abort);
+                if (!ok) break;
+                const int n = __shfl_sync(0xffffffffu, ctl.n_steps[table], 0);
+                more = __shfl_sync(0xffffffffu, ctl.more[table], 0);
+                int place = 0;  // of a step in its stage
+                uint32_t to = 0, bar = 0;
+#pragma unroll 1
+                for (int i = 0; i < n; i++) {
+                    if (place == 0) {
+                        if (!take()) break;
+                        to = dst;
+                        bar = lead_bar<PAIR>(full0 + 8 * stage);
+                    }
+                    const int4 step = ctl.steps[table][i];
+                    const int u_n = __shfl_sync(0xffffffffu, (step.w >> 16) / CTAS, 0);
+                    mbar_expect_more_on(full0 + 8 * stage, (uint32_t)(v_rows * U_RANKS * 2 + u_n * U_BYTES) * CTAS, on_lead);
+                    if (v_rows == VT) {
+                        tma_3d<PAIR>(to, &maps.b[0], 0, step.x + v0 / 4, step.y, bar, on);
+                    } else {
+#pragma unroll 1
+                        for (int m = 1, r = 0; m < 4; m++) {
+                            if (v_rows & VT >> m) {
+                                tma_3d<PAIR>(to + r * 128, &maps.b[m], 0, step.x + v0 / 4 + r, step.y, bar, on);
+                                r += (VT >> m) / 4;
+                            }
+                        }
+                    }
+#pragma unroll 1
+                    for (int r = 0; r < u_n; r += a.u_box)  // two rows of u to 128 bytes
+                        tma_2d<PAIR>(to + B_BYTES + r * U_BYTES, &maps.u, 0, (step.z + half * u_n + r) / 2, bar, on);
+                    to += (uint32_t)a.pack_bytes;
+                    if (++place == a.pack || i == n - 1) {
+                        mbar_arrive_on(full0 + 8 * stage, on_lead);
+                        place = 0;
                         advance();
                     }
-                    wait_for_front();
-                    asm volatile("fence.proxy.async.global;" ::: "memory");
-                    for (int i = 0; i < ahead; i++) load_x(i, i);
                 }
-                for (; s < a.w_steps; s++) {
-                    if (!take()) break;
-                    load_w(s);
-                    load_x(s, stage);
-                    advance();
-                }
-                if (!ok || !a.slots_on) continue;
-                if (!behind) {
-                    wait_for_front();
-                    asm volatile("fence.proxy.async.global;" ::: "memory");
-                }
-                HeadPacks<PAIR> packs(a, row_tile);
-                HeadSlot slot[MAX_PACK];
-                int chunk[MAX_PACK], u_bytes;
-                while (const int n = packs.next(slot, chunk, &u_bytes)) {
-                    if (!take()) break;
-                    const uint32_t dst = base + (uint32_t)(stage * a.stage_bytes), bar = lead_bar<PAIR>(&ctl.full[stage]);
-                    expect(n * v_rows * U_RANKS * 2 + u_bytes);
-                    uint32_t u_dst = dst + A_BYTES;
-#pragma unroll
-                    for (int i = 0; i < MAX_PACK; i++) {
-                        if (i >= n) continue;
-                        const uint32_t b_dst = dst + (uint32_t)(i * B_BYTES);
-                        const int row = chunk[i] * a.b_rows + v0 / 4;  // four vocabulary rows to 128 bytes
-                        if (v_rows == VT) {
-                            tma_3d<PAIR>(b_dst, &maps.b, 0, row, slot[i].adapter, bar);
-                        } else {
-                            for (int r = 0; r < v_rows / 4; r += UNIT / 4)
-                                tma_3d<PAIR>(b_dst + r * 128, &maps.b16, 0, row + r, slot[i].adapter, bar);
-                        }
-                        const int u_n = slot[i].n / CTAS, u_row = chunk[i] * a.u_rows + slot[i].u_row + half * u_n;
-                        for (int r = 0; r < u_n; r += a.u_box)  // two rows of u to 128 bytes
-                            tma_2d<PAIR>(u_dst + r * U_BYTES, &maps.u, 0, (u_row + r) / 2, bar);
-                        u_dst += (uint32_t)(u_n * U_BYTES);
-                    }
-                    advance();
-                }
+                if (ok) mbar_arrive_on(smem_u32(&ctl.steps_empty[table]), on);
             }
-            // every copy has landed before the CTA may end, whether its stage was used or not
-            if (ok) {
-                for (int i = 0; i < a.stages; i++) {  // (a stage never filled counts as empty)
-                    if (!take()) break;
-                    advance();
-                }
+        }
+        // every copy has landed before the CTA may end, whether its stage was used or not
+        if (ok) {
+            for (int i = 0; i < a.stages; i++) {  // (a stage never filled counts as empty)
+                if (!take()) break;
+                advance();
             }
-            if (!ok) {
-                const int outstanding = min(fill, a.stages);
-                for (int i = fill - outstanding; i < fill; i++)
-                    mbar_wait(&ctl.full[i % a.stages], (uint32_t)(i / a.stages) & 1, 100000000ull);
-            }
+        }
+        if (!ok && on) {
+            // the last fill of every stage in use: of this turn of the ring before `stage`, of the turn before from there on
+            for (int i = 0; i < filled; i++)
+                mbar_wait(&ctl.full[i], (i < stage ? phase : phase ^ 1) ^ 1, 100000000ull);
         }
         __syncwarp();
     } else if (warp == WRITERS / 32 + 1) {
-        if (lane == 0 && lead) {
-            int stage = 0, round = 0;
-            uint32_t phase = 0;
+        if (lead) {
+            const bool on = lane == 0;
+            const uint32_t acc_full0 = smem_u32(ctl.acc_full), acc_empty0 = smem_u32(ctl.acc_empty);
+            int stage = 0, round = 0, segment = 0;
+            uint32_t phase = 0, src = base;
             bool ok = true;
             auto take = [&]() {
-                ok = head_wait(&ctl.full[stage], phase, &ctl.abort);
+                ok = warp_wait(full0 + 8 * stage, phase, &ctl.abort);
                 tmem_fence_after();
                 return ok;
             };
             auto advance = [&]() {
-                mma_commit<PAIR>(&ctl.empty[stage]);
-                if (++stage == a.stages) stage = 0, phase ^= 1;
+                mma_commit<PAIR>(empty0 + 8 * stage, on);
+                src += (uint32_t)a.stage_bytes;
+                if (++stage == a.stages) stage = 0, phase ^= 1, src = base;
             };
             uint32_t acc = 0;
             auto begin_round = [&]() {
-                ok = head_wait(&ctl.acc_empty[round & 1], ((round >> 1) & 1) ^ 1, &ctl.abort);
+                ok = warp_wait(acc_empty0 + 8 * (round & 1), ((round >> 1) & 1) ^ 1, &ctl.abort);
                 tmem_fence_after();
                 acc = tmem + (uint32_t)(round & 1) * MAX_COLS;
                 return ok;
             };
-            auto end_round = [&]() { mma_commit<PAIR>(&ctl.acc_full[round++ & 1]); };
+            auto end_round = [&]() {
+                mma_commit<PAIR>(acc_full0 + 8 * (round & 1), on);
+                round++;
+            };
             const uint32_t shape = E4M3 ? shape_e4m3<PAIR>(a.tile_cols) : shape_bf16<PAIR>(a.tile_cols);
-            const uint64_t zero = operand(blocks(U_RANKS * 16), zeros);
             while (ok && tiles.next(&v0, &v_rows, &row_tile)) {
-                for (int s = 0; s < a.w_steps; s++) {
-                    const bool first = s % ROUND == 0;
-                    if (first && !begin_round()) break;
-                    if (!take()) break;
-                    const uint32_t src = base + (uint32_t)(stage * a.stage_bytes);
+                for (int s0 = 0; s0 < a.w_steps; s0 += ROUND) {
+                    if (!begin_round()) break;
+                    const int s1 = min(s0 + ROUND, a.w_steps);
+#pragma unroll 1
+                    for (int s = s0; s < s1; s++) {
+                        if (!take()) break;
+                        const uint32_t w_lo = operand_lo(SWIZZLED_ROWS_LO, src), x_lo = operand_lo(SWIZZLED_ROWS_LO, src + A_BYTES);
 #pragma unroll
-                    for (int k = 0; k < STEP_BYTES; k += 32) {
-                        mma<PAIR, E4M3>(acc, operand(SWIZZLED_ROWS, src + k), operand(SWIZZLED_ROWS, src + A_BYTES + k), shape, !first || k > 0);
+                        for (int k = 0; k < STEP_BYTES / 32; k++)
+                            mma<PAIR, E4M3>(acc, w_lo + 2 * k, SWIZZLED_ROWS_HI, x_lo + 2 * k, SWIZZLED_ROWS_HI, shape, k > 0 || s > s0, on);
+                        advance();
                     }
-                    advance();
-                    if (s % ROUND == ROUND - 1 || s == a.w_steps - 1) {
-                        if (!(a.slots_on && !own_round && s == a.w_steps - 1)) end_round();
-                    }
+                    if (!ok) break;
+                    if (s1 < a.w_steps || !a.slots_on || own_round) end_round();
                 }
                 if (!ok || !a.slots_on) continue;
-                wait_for_front();
-                HeadPacks<PAIR> packs(a, row_tile);
                 if (own_round) {
-                    if (packs.at == packs.end) continue;
                     if (!begin_round()) break;
-                    // the slots' windows may cover a tile in part only: zero times zero first
-                    mma<PAIR, false>(acc, zero, zero, shape_bf16<PAIR>(a.tile_cols), false);
+                    // the slots' windows may cover a tile in part only, or not at all: zero times zero first
+                    const uint32_t lo = operand_lo(BLOCKS_LO, zeros);
+                    mma<PAIR, false>(acc, lo, B_BLOCKS_HI, lo, B_BLOCKS_HI, shape_bf16<PAIR>(a.tile_cols), false, on);
                 }
-                HeadSlot slot[MAX_PACK];
-                int chunk[MAX_PACK], u_bytes;
-                while (const int n = packs.next(slot, chunk, &u_bytes)) {
-                    if (!take()) break;
-                    const uint32_t src = base + (uint32_t)(stage * a.stage_bytes);
-                    uint32_t u_src = src + A_BYTES;
-#pragma unroll
-                    for (int i = 0; i < MAX_PACK; i++) {
-                        if (i >= n) continue;
-                        const uint32_t d = acc + (uint32_t)slot[i].col, n_shape = shape_bf16<PAIR>(slot[i].n);
-                        const uint64_t bd = operand(blocks(U_RANKS * 16), src + (uint32_t)(i * B_BYTES));
-                        mma<PAIR, false>(d, bd, operand(blocks(U_BYTES * 8), u_src), n_shape, true);
-                        mma<PAIR, false>(d, bd, operand(blocks(U_BYTES * 8), u_src + 256), n_shape, true);
-                        u_src += (uint32_t)(slot[i].n / CTAS * U_BYTES);
+                bool more = true;
+                for (; ok && more; segment++) {
+                    const int table = segment & 1;
+                    ok = warp_wait(smem_u32(&ctl.steps_full[table]), (segment >> 1) & 1, &ctl.abort);
+                    if (!ok) break;
+                    const int n = __shfl_sync(0xffffffffu, ctl.n_steps[table], 0);
+                    more = __shfl_sync(0xffffffffu, ctl.more[table], 0);
+                    int place = 0;
+                    uint32_t at = 0;
+#pragma unroll 1
+                    for (int i = 0; i < n; i++) {
+                        if (place == 0) {
+                            if (!take()) break;
+                            at = src;
+                        }
+                        const int window = __shfl_sync(0xffffffffu, ctl.steps[table][i].w, 0);
+                        const uint32_t d = acc + (uint32_t)(window & 0xffff), n_shape = shape_bf16<PAIR>(window >> 16);
+                        const uint32_t b_lo = operand_lo(BLOCKS_LO, at), u_lo = operand_lo(BLOCKS_LO, at + B_BYTES);
+                        mma<PAIR, false>(d, b_lo, B_BLOCKS_HI, u_lo, U_BLOCKS_HI, n_shape, true, on);             // leading parts
+                        mma<PAIR, false>(d, b_lo, B_BLOCKS_HI, u_lo + (256 >> 4), U_BLOCKS_HI, n_shape, true, on);  // remainders
+                        at += (uint32_t)a.pack_bytes;
+                        if (++place == a.pack || i == n - 1) {
+                            place = 0;
+                            advance();
+                        }
                     }
-                    advance();
+                    if (ok) mbar_arrive_on(smem_u32(&ctl.steps_empty[table]), on);
                 }
                 if (ok) end_round();
             }
             if (!ok) {  // what was issued ends before tensor memory is given back
-                mma_commit<PAIR>(&ctl.drain);
-                mbar_wait(&ctl.drain, 0, 100000000ull);
+                mma_commit<PAIR>(smem_u32(&ctl.drain), on);
+                if (on) mbar_wait(&ctl.drain, 0, 100000000ull);
+            }
+        }
+        __syncwarp();
+    } else if (warp == WRITERS / 32 + 2) {
+        if (a.slots_on) {
+            wait_for_front();
+            bool ok = true;
+            int segment = 0;
+            while (ok && tiles.next(&v0, &v_rows, &row_tile)) {
+                const int first = a.tile_first[row_tile], total = (a.tile_first[row_tile + 1] - first) * a.chunks;
+                int at = 0;
+                do {  // (a tile without adapters: one segment of nothing)
+                    const int table = segment & 1, n = min(SEGMENT, total - at);
+                    int free = 1;
+                    if (lane == 0) free = head_wait(&ctl.steps_empty[table], ((segment >> 1) & 1) ^ 1, &ctl.abort);
+                    ok = __shfl_sync(0xffffffffu, free, 0);
+                    if (!ok) break;
+                    for (int i = lane; i < n; i += 32) {
+                        const HeadSlot slot = a.slots[first + (at + i) / a.chunks];
+                        const int chunk = (at + i) % a.chunks;
+                        ctl.steps[table][i] = make_int4(chunk * a.b_rows, slot.adapter, chunk * a.u_rows + slot.u_row, slot.col | slot.n << 16);
+                    }
+                    at += n;
+                    if (lane == 0) {
+                        ctl.n_steps[table] = n;
+                        ctl.more[table] = at < total;
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&ctl.steps_full[table]);
+                    segment++;
+                } while (at < total);
             }
         }
         __syncwarp();
@@ -545,11 +620,7 @@ __global__ void __launch_bounds__(HEAD_NT, 1) head_rows_kernel(const HeadArgs a,
                     }
                 }
             }
-            int rounds = w_rounds;
-            if (own_round) {
-                wait_for_front();
-                rounds += a.tile_first[row_tile] < a.tile_first[row_tile + 1];
-            }
+            const int rounds = w_rounds + own_round;
             for (int r = 0; r < rounds && ok; r++, round++) {
                 // one lane of a warp watches the barrier
                 int landed = 1;

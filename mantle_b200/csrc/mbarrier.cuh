@@ -17,17 +17,18 @@ constexpr uint64_t WAIT_LIMIT_NS = 2000000000ull;  // 2 s
 // One poll.  The suspend-time hint lets the hardware park the thread until the phase completes
 // (or the hint, in nanoseconds, runs out) instead of spinning through issue slots that the
 // other CTA on the SM could use.
-__device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
+__device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
     uint32_t ok;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
         "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
         "selp.u32 %0, 1, 0, p;\n\t}"
         : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity), "r"(WAIT_HINT_NS)
+        : "r"(bar), "r"(parity), "r"(WAIT_HINT_NS)
         : "memory");
     return ok != 0;
 }
+__device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) { return mbar_try_wait(smem_u32(bar), parity); }
 
 __device__ __forceinline__ uint64_t global_ns() {
     uint64_t t;
