@@ -32,6 +32,7 @@
 #include <stdint.h>
 
 #include "mantle_cuda_sampler.h"
+#include "mantle_head.h"
 
 #ifdef __cplusplus
 extern "C" {
@@ -79,6 +80,17 @@ int mantleBatchSamplerCanUseDeviceGreedy(const MantleBatchSampler* s, int row);
  */
 int mantleBatchSamplerStep(MantleBatchSampler* s, const void* dev_logits, int dtype, int64_t row_stride,
                            const double* uniforms, float logit_scale, float logit_softcap, mantleCudaStream_t stream);
+
+/*
+ * The same from the hidden state of the model's last layer: the norm (`norm` may be NULL), the head with the
+ * adapters of the rows' requests, and the step on the logits it writes, one behind the other on `stream`.
+ * head->rows and head->vocab are the sampler's, norm->out is what the head reads (hidden_rows), with the same
+ * rows, width, type, stride and scales; workspace as for mantleCudaHeadRows.  cudaErrorInvalidValue, with
+ * nothing launched, where any of it does not fit.
+ */
+int mantleBatchSamplerStepHidden(MantleBatchSampler* s, const MantleNormBatch* norm, const MantleHeadBatch* head,
+                                 void* workspace, size_t workspace_bytes, const double* uniforms, float logit_scale,
+                                 float logit_softcap, mantleCudaStream_t stream);
 
 /*
  * The last step's results, valid once `stream` has been synchronised and until the next Step:

@@ -291,7 +291,8 @@ int mantleCudaSampleRowsNoAlloc(const MantleSampleBatch* batch, mantleCudaStream
 /* Size of the static scratch behind mantleCudaSampleRowsNoAlloc. */
 size_t mantleCudaSamplerStaticScratchBytes(void);
 
-/* Text of the last refusal of mantleCudaSampleRowsNoAlloc on the calling thread ("" if none). */
+/* Text of the last refusal of mantleCudaSampleRowsNoAlloc, or of a call of mantle_head.h, on the calling thread
+ * ("" if none). */
 const char* mantleCudaSamplerLastError(void);
 
 /*

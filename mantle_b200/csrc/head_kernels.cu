@@ -260,6 +260,8 @@ int launch_head(const HeadArgs& a, const HeadMaps& maps, const HeadLayout& l, cu
 
 }  // namespace
 
+const char* mantle_internal_norm_fault(const MantleNormBatch* b) { return norm_fault(b); }
+
 extern "C" int mantleCudaNormRows(const MantleNormBatch* b, mantleCudaStream_t stream_) {
     const char* fault = norm_fault(b);
     if (fault) return refuse(fault);

@@ -249,6 +249,34 @@ extern "C" int mantleBatchSamplerStep(MantleBatchSampler* s, const void* dev_log
     return (int)e;
 }
 
+extern "C" int mantleBatchSamplerStepHidden(MantleBatchSampler* s, const MantleNormBatch* norm, const MantleHeadBatch* head,
+                                            void* workspace, size_t workspace_bytes, const double* uniforms,
+                                            float logit_scale, float logit_softcap, mantleCudaStream_t stream) {
+    if (!s || !head || !uniforms) return kInvalid;
+    size_t need = 0;
+    int rc = mantleCudaHeadWorkspaceBytes(head, &need);  // checks the whole batch
+    if (rc) return rc;
+    const char* fault = norm ? mantle_internal_norm_fault(norm) : nullptr;
+    if (!fault && need && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 256))
+        fault = "head: the workspace is missing, too small or not on 256 bytes";
+    if (!fault && (head->rows != s->rows || head->vocab != s->vocab))
+        fault = "the head's rows and vocabulary are not the batch sampler's";
+    if (!fault && norm && (norm->out != head->hidden_rows || norm->rows != head->rows || norm->hidden != head->hidden ||
+                           norm->out_dtype != head->dtype || norm->out_stride != head->hidden_stride))
+        fault = "the head does not read what the norm writes";
+    if (!fault && norm && norm->out_scale && (norm->out_scale != head->hidden_scales || norm->scale_group != 0 || norm->scale_stride != 1))
+        fault = "the head wants the norm's scales, one a row and one behind the other";
+    if (fault) {
+        mantle_internal_set_last_error(fault);
+        return kInvalid;
+    }
+    rc = norm ? mantleCudaNormRows(norm, stream) : 0;
+    if (rc) return rc;
+    rc = mantleCudaHeadRows(head, workspace, workspace_bytes, stream);
+    if (rc) return rc;
+    return mantleBatchSamplerStep(s, head->out, head->out_dtype, head->out_stride, uniforms, logit_scale, logit_softcap, stream);
+}
+
 extern "C" int mantleBatchSamplerResults(MantleBatchSampler* s, const int32_t** next, const int32_t** ended,
                                          int32_t* status, const int32_t** dev_next) {
     if (!s) return kInvalid;

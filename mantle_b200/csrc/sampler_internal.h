@@ -3,10 +3,14 @@
 
 #include <string.h>
 
+#include "../../include/mantle_head.h"
 #include "../../include/mantle_sample_params.h"
 
 // Sets the text mantleCudaSamplerLastError() returns on the calling thread.
 __attribute__((visibility("hidden"))) void mantle_internal_set_last_error(const char* msg);
+
+// What is wrong with a norm's batch; nullptr: nothing.
+__attribute__((visibility("hidden"))) const char* mantle_internal_norm_fault(const MantleNormBatch* b);
 
 // NewSampler's normalisation, internal/logits/sampler.go:61-83.
 static inline void mantle_internal_normalise(const MantleSamplerConfig& cfg, MantleSampleParams* p) {

@@ -210,6 +210,9 @@ BATCH_EXPORTS = {
     "mantleBatchSamplerCanUseDeviceGreedy": (C.c_int, [C.c_void_p, C.c_int]),
     "mantleBatchSamplerStep": (
         C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_int64, C.c_void_p, C.c_float, C.c_float, C.c_void_p]),
+    "mantleBatchSamplerStepHidden": (
+        C.c_int, [C.c_void_p, C.POINTER(NormBatch), C.POINTER(HeadBatch), C.c_void_p, C.c_size_t, C.c_void_p, C.c_float, C.c_float,
+                  C.c_void_p]),
     "mantleBatchSamplerResults": (
         C.c_int, [C.c_void_p, C.POINTER(C.c_void_p), C.POINTER(C.c_void_p), C.POINTER(C.c_int32), C.POINTER(C.c_void_p)]),
 }

@@ -555,6 +555,26 @@ class BatchSampler:
                                                  _stream_ptr(stream))
         native.check(rc, "mantleBatchSamplerStep")
 
+    def step_hidden_async(self, head, uniforms, norm=None, stream=None, logit_scale=0.0, logit_softcap=0.0):
+        """Queues norm (head.NormPlan, optional), head (head.HeadPlan) and one step on the logits it writes."""
+        if head.device != self.device or (norm is not None and norm.device != self.device):
+            raise ValueError("the plans are not on %s" % self.device)
+        u = np.ascontiguousarray(uniforms, dtype=np.float64)
+        if u.shape != (self.rows,):
+            raise ValueError("one uniform per row")
+        with torch.cuda.device(self.device):
+            rc = self.lib.mantleBatchSamplerStepHidden(
+                self.handle, None if norm is None else C.byref(norm.batch), C.byref(head.batch), _ptr(head.workspace),
+                head.workspace_bytes, u.ctypes.data_as(C.c_void_p), logit_scale, logit_softcap, _stream_ptr(stream))
+        native.check(rc, "mantleBatchSamplerStepHidden")
+
+    def step_hidden(self, head, rngs, **kw):
+        """step() from the hidden state that `head` (behind `norm`) reads."""
+        self.step_hidden_async(head, self.draw(rngs), **kw)
+        torch.cuda.current_stream(self.device).synchronize()
+        n, e, status = self.results()
+        return n, e
+
     def results(self):
         """(next tokens, ended flags, status word) of the last step, as numpy arrays (copies)."""
         nxt, end, dev = C.c_void_p(), C.c_void_p(), C.c_void_p()

@@ -318,3 +318,79 @@ def test_norm_head_sampler_in_a_row():
     R.check(plan.out, want, slack)
     ref = O.sample_rows(plan.out.cpu().numpy(), params)
     assert np.array_equal(out.next.cpu().numpy(), ref["next"])
+
+
+def test_decode_loop_from_the_hidden_state():
+    """BatchSampler.step_hidden: the tokens are those of a BatchSampler that is fed the head's logits, step after step."""
+    rows, vocab, hidden = 20, 4001, 256
+    s = head_inputs(rows, vocab, hidden, BF16, 5, 8)
+    x, r = rand(1, rows, hidden).to(BF16), rand(2, rows, hidden).to(BF16)
+    norm = H.NormPlan(x, rand(3, hidden).to(BF16), residual=r, weight_offset=1.0, out=s["hidden"])
+    plan = head_plan(s)
+    both = [sampler.BatchSampler(rows, vocab, 64, [7], device=DEV) for _ in range(2)]
+    for i in range(rows):
+        cfg = sampler.SamplerConfig(seed=i, temperature=0.9, top_k=20, top_p=0.95, repeat_penalty=1.2, repeat_last_n=16)
+        for b in both:
+            b.set_row(i, cfg, [i, i + 1])
+    rngs = [[np.random.default_rng(i).random for i in range(rows)] for _ in both]
+    for turn in range(6):
+        x.copy_(rand(100 + turn, rows, hidden).to(BF16))
+        s["ids"].copy_(torch.randint(-1, 5, (rows,), generator=torch.Generator().manual_seed(turn), dtype=torch.int32))
+        got, ended = both[0].step_hidden(plan, rngs[0], norm=norm)
+        check_norm(x, norm.keep[1], r, offset=1.0, plan=norm, where=turn)  # (runs the norm again, to the same place)
+        want, slack = R.head(**s)
+        R.check(plan.out, want, slack, turn)
+        ref, ref_ended = both[1].step(plan.out, rngs[1])
+        assert np.array_equal(got, ref) and np.array_equal(ended, ref_ended)
+    other = head_plan(head_inputs(rows, vocab + 1, hidden, BF16))
+    for bad in (dict(head=other), dict(head=plan, norm=H.NormPlan(x)), dict(head=plan, norm=H.NormPlan(x, out_dtype=E4M3))):
+        with pytest.raises(native.CudaError):
+            both[0].step_hidden_async(uniforms=np.zeros(rows), **bad)
+    with pytest.raises(ValueError):
+        both[0].step_hidden_async(plan, np.zeros(rows + 1))
+    for b in both:
+        b.close()
+
+
+def test_an_adapter_is_replaced():
+    s = head_inputs(30, 700, 128, BF16, 4, 16)
+    ad = H.Adapters(s["a"], s["b"], s["gain"])
+    plan = H.HeadPlan(s["hidden"], s["weight"], adapters=ad, adapter_ids=s["ids"])
+    t = head_inputs(30, 700, 128, BF16, 4, 16, seed=50)
+    s["b"] = s["b"].clone()
+    ad.replace(2, t["a"][1], t["b"][1], 1.75)
+    s["b"][2] = t["b"][1]
+    check_head(s, plan=plan)
+    assert torch.equal(s["a"][2], t["a"][1]) and float(s["gain"][2]) == 1.75
+    with pytest.raises(ValueError):
+        ad.replace(4, t["a"][1], t["b"][1], 1.0)
+    with pytest.raises(ValueError):
+        ad.replace(1, t["a"][1], t["b"][1])
+
+
+def test_plans_refuse_what_they_cannot_run():
+    s = head_inputs(8, 100, 64, BF16, 2, 8)
+    x = s["hidden"]
+    ad = H.Adapters(s["a"], s["b"])
+    for args, kw in (((x,), {}), ((x, s["weight"]), dict(base=torch.zeros(8, 100, device=DEV))),
+                     ((x, s["weight"][:, :32]), {}), ((x, s["weight"]), dict(adapters=ad)),
+                     ((x, s["weight"]), dict(adapter_ids=s["ids"])), ((x, s["weight"]), dict(adapters=ad, adapter_ids=s["ids"].long())),
+                     ((x, s["weight"]), dict(adapters=ad, adapter_ids=s["ids"][:7])), ((x, s["weight"][:50]), dict(adapters=ad, adapter_ids=s["ids"])),
+                     ((x, s["weight"]), dict(out_dtype=torch.float16)), ((x, s["weight"]), dict(out=torch.zeros(8, 99, device=DEV))),
+                     ((x, s["weight"]), dict(hidden_scales=torch.ones(8, device=DEV))), ((x.float(), s["weight"]), {}),
+                     ((x.to(E4M3), s["weight"].to(E4M3)), {})):
+        with pytest.raises(ValueError):
+            H.HeadPlan(*args, **kw)
+    with pytest.raises(native.CudaError, match="16 bytes"):  # rows of W that TMA cannot read
+        H.HeadPlan(x[:, :56].contiguous(), torch.zeros(100, 60, device=DEV, dtype=BF16)[:, :56])
+    with pytest.raises(native.CudaError, match="multiple of 8"):
+        H.HeadPlan(x[:, :60].contiguous(), torch.zeros(100, 60, device=DEV, dtype=BF16))
+    wide = torch.zeros(8, 200, device=DEV, dtype=BF16)
+    with pytest.raises(ValueError, match="overlaps"):
+        H.NormPlan(wide[:, :64], out=wide[:, 32:96])
+    with pytest.raises(ValueError, match="overlaps"):
+        H.HeadPlan(wide[:, :64], s["weight"], out_dtype=BF16, out=wide[:, 100:])
+    with pytest.raises(ValueError):
+        H.NormPlan(wide, residual=wide.float())
+    with pytest.raises(native.CudaError, match="MAX_HIDDEN"):
+        H.NormPlan(torch.zeros(1, 32769, device=DEV)).launch()

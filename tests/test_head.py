@@ -152,3 +152,18 @@ def test_definitions_against_elementary_sums():
                 t += float(gain[n]) * sum(float(b[n, v, j]) * sum(float(a[n, j, k]) * float(x[i, k]) for k in range(6)) for j in range(3))
             assert abs(float(out[i, v]) - t) < 1e-12
     assert bool((slack > 0).all())
+
+
+def test_pack_and_step_refusals():
+    lib = native.load()
+    n = C.c_size_t(7)
+    for args in ((0, 10, 8), (1, 0, 8), (1, 10, 0), (1, 10, 12), (1, 10, 264), (4097, 10, 8), (1, native.MAX_VOCAB + 1, 8)):
+        assert lib.mantleCudaAdapterPackBytes(*args, C.byref(n)) == INV
+        assert lib.mantleCudaAdapterPack(0x1000, *args, 0x2000, None) == INV
+    assert n.value == 7
+    assert lib.mantleCudaAdapterPackBytes(2, 257, 24, C.byref(n)) == 0 and n.value == 2 * 2 * 512 * 16 * 2
+    assert lib.mantleCudaAdapterPack(None, 1, 10, 8, 0x2000, None) == INV
+    assert lib.mantleCudaAdapterPack(0x1000, 1, 10, 8, None, None) == INV
+    assert lib.mantleCudaAdapterPack(0x1008, 1, 10, 8, 0x2000, None) == INV
+    assert lib.mantleCudaAdapterPack(0x1000, 1, 10, 8, 0x2040, None) == INV
+    assert lib.mantleBatchSamplerStepHidden(None, None, C.byref(head_batch()), None, 0, None, 0.0, 0.0, None) == INV
