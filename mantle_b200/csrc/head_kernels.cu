@@ -220,7 +220,7 @@ bool encode_plain(CUtensorMap* m, const void* p, long long d1, long long d2, int
 }
 
 template <class... Args>
-int launch(void (*kern)(Args...), dim3 grid, int threads, size_t smem, cudaStream_t stream, bool dependent, bool pair, Args... args) {
+int launch(void (*kern)(Args...), dim3 grid, int threads, size_t smem, cudaStream_t stream, bool pair, Args... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = dim3((unsigned)threads);
@@ -228,10 +228,9 @@ int launch(void (*kern)(Args...), dim3 grid, int threads, size_t smem, cudaStrea
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     cfg.attrs = attr;
-    if (dependent) {
-        attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
-    }
+    // every kernel here waits for what is in front of it by itself (griddepcontrol.wait), after its own set-up
+    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
     if (pair) {
         attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
         attr[cfg.numAttrs].val.clusterDim.x = 2;
@@ -247,7 +246,7 @@ int launch_head_as(const HeadArgs& a, const HeadMaps& maps, const HeadLayout& l,
     const auto kern = head_rows_kernel<E4M3, OUT16, GROUPS>;
     const int rc = ensure_smem(kern, l.smem, granted);
     if (rc) return rc;
-    return launch<HeadArgs, HeadMaps>(kern, dim3((unsigned)l.grid), HEAD_NT, l.smem, stream, l.adapters || l.copied, l.pair, a, maps);
+    return launch<HeadArgs, HeadMaps>(kern, dim3((unsigned)l.grid), HEAD_NT, l.smem, stream, l.pair, a, maps);
 }
 
 template <bool E4M3, bool OUT16>
@@ -346,6 +345,7 @@ extern "C" int mantleCudaHeadRows(const MantleHeadBatch* b, void* workspace, siz
     a.tile_cols = l.tile_cols;
     a.row_tiles = l.row_tiles;
     a.v_tiles = l.v_tiles;
+    a.front_is_ours = l.adapters || l.copied;
     a.slots_on = l.adapters;
     a.sorted = l.sorted;
     a.copied = l.copied;
@@ -418,13 +418,13 @@ extern "C" int mantleCudaHeadRows(const MantleHeadBatch* b, void* workspace, siz
 
     int rc = 0;
     if (l.sorted) {
-        rc = launch<HeadPrep>(head_sort_kernel, dim3(1), SORT_NT, ((size_t)b->n_adapters + 1) * 4, stream, false, false, p);
+        rc = launch<HeadPrep>(head_sort_kernel, dim3(1), SORT_NT, ((size_t)b->n_adapters + 1) * 4, stream, false, p);
         if (rc) return rc;
     }
     if (l.adapters || l.copied) {
         const dim3 grid((unsigned)(p.units + p.copy_ctas), (unsigned)std::max(1, l.chunks));
-        rc = l.sorted ? launch<HeadPrep>(head_shrink_kernel, grid, SHRINK_NT, 0, stream, true, false, p)
-                      : launch<HeadPrep>(head_shrink_here_kernel, grid, SHRINK_NT, 0, stream, false, false, p);
+        rc = l.sorted ? launch<HeadPrep>(head_shrink_kernel, grid, SHRINK_NT, 0, stream, false, p)
+                      : launch<HeadPrep>(head_shrink_here_kernel, grid, SHRINK_NT, 0, stream, false, p);
         if (rc) return rc;
     }
     if (b->out_dtype == MANTLE_DTYPE_BF16)

@@ -92,8 +92,9 @@ __device__ __forceinline__ int block_scan(int v, int* warp_sums, int* total) {
 __global__ void __launch_bounds__(SORT_NT) head_sort_kernel(const HeadPrep p) {
     extern __shared__ int bins[];  // [n_adapters + 1]: counts, then next free places, then ends of runs
     __shared__ int warp_sums[32];
-    pdl_trigger();
     const int n = p.n_adapters, tid = threadIdx.x;
+    pdl_wait();
+    pdl_trigger();
     for (int b = tid; b <= n; b += SORT_NT) bins[b] = 0;
     __syncthreads();
     for (int r = tid; r < p.rows; r += SORT_NT) {
@@ -293,8 +294,8 @@ __device__ __forceinline__ void store_u(const HeadPrep& p, int rank_at, int u_ro
 __global__ void __launch_bounds__(SHRINK_NT) head_shrink_kernel(const HeadPrep p) {
     __shared__ ShrinkSums sums;
     __shared__ int rows[WINDOW];
-    pdl_trigger();
     pdl_wait();
+    pdl_trigger();
     if ((int)blockIdx.x >= p.units) {
         if (blockIdx.y == 0)
             copy_rows(p, ((int)blockIdx.x - p.units) * SHRINK_WARPS + (int)(threadIdx.x >> 5), p.copy_ctas * SHRINK_WARPS);
@@ -320,7 +321,8 @@ __global__ void __launch_bounds__(SHRINK_NT) head_shrink_here_kernel(const HeadP
     __shared__ __align__(16) int ids[HERE_ROWS];
     __shared__ int mine[HERE_ROWS], first_of[HERE_ROWS];
     __shared__ int counts[2 * (HERE_ROWS / 32)];
-    pdl_trigger();
+    pdl_wait();
+    pdl_trigger();  // not before: the projection reads W and x as soon as it starts
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if ((int)blockIdx.x >= p.units) {
         if (blockIdx.y == 0)

@@ -8,13 +8,14 @@
 // writes 32 neighbouring columns of a row of logits per warp.  W and B pass through the SM once per tile of
 // rows, whatever the number of rows.
 //
-// One CTA per SM, persistent over its tiles.  Warp 8 moves operands with TMA into a ring of stages (a stage: 128
-// rows of W, 128 bytes wide, and the same slice of x; or some adapters' B, 16 ranks wide, and their windows of u),
-// warp 9 issues tcgen05.mma from it, warps 0-7 read accumulators out of tensor memory, add them up in registers
-// and write the finished tile while the next one is computed.  Warp 10 works out, a lane each, what every step of the
-// tile's adapters copies and multiplies, ahead of warps 8 and 9, whose single threads then do little but issue:
-// instructions that are not a short loop cost such a thread ten to twenty cycles each (with slots read from L2 and
-// steps worked out by the issuing threads 16 adapters cost 64 rows 53 us, TODO us now).
+// One CTA per SM, persistent over its tiles.  Warps 8 and 11 move operands with TMA into a ring of stages: warp 8 what
+// depends on the vocabulary (128 rows of W, 128 bytes wide; or some adapters' B, 16 ranks wide), warp 11 what depends on
+// the batch (the same slice of x, or the windows of u).  Warp 9 issues tcgen05.mma from the ring, warps 0-7 read
+// accumulators out of tensor memory, add them up in registers and write the finished tile while the next one is
+// computed.  Warp 10 works out, a lane each, what every step of the tile's adapters copies and multiplies, ahead of the
+// three that issue: an instruction that starts a copy or a product costs its warp some hundred cycles, and what
+// stands around it comes on top (one adapter's step of 64 rows: 490 cycles to copy and 380 to multiply; it has
+// 4 KB of B, which HBM delivers in 170).
 //
 // Pairs.  W comes from HBM once, but x from L2 for every 128 vocabulary rows: at 256 rows that is twice W's bytes,
 // and what L2 can hand out (about 10 TB/s) bounds the kernel long before HBM or the tensor cores do.  From 65 rows
@@ -45,7 +46,7 @@ constexpr int B_BYTES = VT * U_RANKS * 2;  // one adapter's B of one chunk and a
 constexpr int ROUND_BF16 = 8;      // steps of a round
 constexpr int ROUND_E4M3 = 64;
 constexpr int WRITERS = 256;       // threads that read accumulators and write results
-constexpr int HEAD_NT = WRITERS + 96;
+constexpr int HEAD_NT = WRITERS + 128;
 constexpr int ZERO_BYTES = VT * 32;
 constexpr int SEGMENT = 96;        // adapters' steps that are worked out at a time; a multiple of 2, 3 and 4
 
@@ -61,6 +62,7 @@ struct __align__(16) HeadCtl {
 
 struct HeadArgs {
     int rows, vocab, w_steps, tile_cols, row_tiles, v_tiles;
+    int front_is_ours;                // prepare kernels of the same call stand in front
     int slots_on, sorted, copied;  // adapters; perm and x come from the kernel in front
     int chunks, u_rows, u_box;        // u_box: rows of u of one copy
     int pack, pack_bytes;             // adapters' steps in one stage, and the room of each
@@ -312,7 +314,7 @@ __global__ void __launch_bounds__(HEAD_NT, 1) head_rows_kernel(const HeadArgs a,
     }
     if (threadIdx.x == 0) {
         for (int s = 0; s < a.stages; s++) {
-            mbar_init(&ctl.full[s], 1);
+            mbar_init(&ctl.full[s], 2);  // the announcements of warps 8 and 11
             mbar_init(&ctl.empty[s], 1);
         }
         for (int i = 0; i < 2; i++) {
@@ -321,7 +323,7 @@ __global__ void __launch_bounds__(HEAD_NT, 1) head_rows_kernel(const HeadArgs a,
         }
         for (int i = 0; i < 2; i++) {
             mbar_init(&ctl.steps_full[i], 1);
-            mbar_init(&ctl.steps_empty[i], lead ? 2 : 1);
+            mbar_init(&ctl.steps_empty[i], lead ? 3 : 2);
         }
         mbar_init(&ctl.drain, 1);
         ctl.abort = 0;
@@ -341,6 +343,9 @@ __global__ void __launch_bounds__(HEAD_NT, 1) head_rows_kernel(const HeadArgs a,
     sync_all<PAIR>();
     tmem_fence_after();
     const uint32_t tmem = ctl.tmem;
+    // Launched before the kernel in front has ended, so that all this overlaps its end.  That kernel is this call's own
+    // (which starts no earlier than what was in front of it has ended) or, without prepare kernels, anybody's.
+    if (!a.front_is_ours) pdl_wait();
     HeadTiles<PAIR> tiles(a);
     int v0, v_rows, row_tile;
     // what the kernels in front wrote may be read from here on (each thread asks once, where it first needs it)
@@ -350,63 +355,69 @@ __global__ void __launch_bounds__(HEAD_NT, 1) head_rows_kernel(const HeadArgs a,
         behind = true;
     };
     const uint32_t full0 = smem_u32(ctl.full), empty0 = smem_u32(ctl.empty);  // barriers of stage 0, 8 bytes each
-    if (warp == WRITERS / 32) {
+    if (warp == WRITERS / 32 || warp == WRITERS / 32 + 3) {
+        const bool v_side = warp == WRITERS / 32;  // W and B; else x and u
         const bool on = lane == 0, on_lead = on && lead;
         const int x_rows = a.tile_cols / CTAS, half = PAIR ? blockIdx.x & 1 : 0;
-        const uint32_t step_bytes = (uint32_t)a.stage_bytes;
+        const uint32_t stage_bytes = (uint32_t)a.stage_bytes;
         int filled = 0, stage = 0, segment = 0;  // filled: stages in use so far
         uint32_t phase = 1, dst = base;          // phase of `empty`: the first round passes
         bool ok = true;
         auto take = [&]() { return ok = warp_wait(empty0 + 8 * stage, phase, &ctl.abort); };
         auto advance = [&]() {
             filled = max(filled, ++stage);
-            dst += step_bytes;
+            dst += stage_bytes;
             if (stage == a.stages) stage = 0, phase ^= 1, dst = base;
         };
-        auto load_w = [&](int s) {
-            const uint32_t bar = lead_bar<PAIR>(full0 + 8 * stage);
-            // the even CTA of a pair awaits the bytes of both; a barrier counts them in any order
-            mbar_expect_on(full0 + 8 * stage, (uint32_t)((v_rows + x_rows) * STEP_BYTES * CTAS), on_lead);
+        // v_rows vocabulary rows in as few copies as their sizes allow
+        auto copy_w = [&](int x, uint32_t bar) {
             if (v_rows == VT) {
-                tma_2d<PAIR>(dst, &maps.w[0], s * STEP_COLS, v0, bar, on);
+                tma_2d<PAIR>(dst, &maps.w[0], x, v0, bar, on);
                 return;
             }
 #pragma unroll 1
             for (int m = 1, v = 0; m < 4; m++) {
                 if (v_rows & VT >> m) {
-                    tma_2d<PAIR>(dst + v * STEP_BYTES, &maps.w[m], s * STEP_COLS, v0 + v, bar, on);
+                    tma_2d<PAIR>(dst + v * STEP_BYTES, &maps.w[m], x, v0 + v, bar, on);
                     v += VT >> m;
                 }
             }
         };
-        auto load_x = [&](int s, int st, uint32_t to) {
-            tma_2d<PAIR>(to + A_BYTES, &maps.x, s * STEP_COLS, row_tile * a.tile_cols + half * x_rows, lead_bar<PAIR>(full0 + 8 * st), on);
-        };
-        while (ok && tiles.next(&v0, &v_rows, &row_tile)) {
-            int s = 0;
-            if (a.copied && !behind) {
-                // W does not come from the kernels in front: the ring fills with it while they still run
-                const int ahead = min(a.stages, a.w_steps);
-                for (; s < ahead; s++) {
-                    load_w(s);
-                    advance();
-                }
-                wait_for_front();
-                asm volatile("fence.proxy.async.global;" ::: "memory");
-                for (int i = 0; i < ahead; i++) load_x(i, i, base + i * step_bytes);
+        auto copy_b = [&](int row, int adapter, uint32_t to, uint32_t bar) {  // four vocabulary rows to 128 bytes
+            if (v_rows == VT) {
+                tma_3d<PAIR>(to, &maps.b[0], 0, row, adapter, bar, on);
+                return;
             }
 #pragma unroll 1
-            for (; s < a.w_steps; s++) {
-                if (!take()) break;
-                load_w(s);
-                load_x(s, stage, dst);
-                advance();
+            for (int m = 1, r = 0; m < 4; m++) {
+                if (v_rows & VT >> m) {
+                    tma_3d<PAIR>(to + r * 128, &maps.b[m], 0, row + r, adapter, bar, on);
+                    r += (VT >> m) / 4;
+                }
             }
-            if (!ok || !a.slots_on) continue;
+        };
+        auto fence_front = [&]() {
             if (!behind) {
                 wait_for_front();
                 asm volatile("fence.proxy.async.global;" ::: "memory");
             }
+        };
+        // W and B do not come from the kernels in front: their copies start while those still run
+        if (!v_side && a.copied) fence_front();
+        while (ok && tiles.next(&v0, &v_rows, &row_tile)) {
+            // the even CTA of a pair awaits the bytes of both; a barrier counts them in any order
+            const uint32_t bytes = (uint32_t)((v_side ? v_rows : x_rows) * STEP_BYTES * CTAS);
+#pragma unroll 1
+            for (int s = 0; s < a.w_steps; s++) {
+                if (!take()) break;
+                const uint32_t bar = lead_bar<PAIR>(full0 + 8 * stage);
+                mbar_expect_on(full0 + 8 * stage, bytes, on_lead);
+                if (v_side) copy_w(s * STEP_COLS, bar);
+                else tma_2d<PAIR>(dst + A_BYTES, &maps.x, s * STEP_COLS, row_tile * a.tile_cols + half * x_rows, bar, on);
+                advance();
+            }
+            if (!ok || !a.slots_on) continue;
+            if (!v_side) fence_front();
             bool more = true;
             for (; ok && more; segment++) {
                 const int table = segment & 1;
@@ -416,36 +427,32 @@ __global__ void __launch_bounds__(HEAD_NT, 1) head_rows_kernel(const HeadArgs a,
                 more = __shfl_sync(0xffffffffu, ctl.more[table], 0);
                 int place = 0;  // of a step in its stage
                 uint32_t to = 0, bar = 0;
+                int4 step = ctl.steps[table][0];
 #pragma unroll 1
                 for (int i = 0; i < n; i++) {
+                    const int4 next = ctl.steps[table][min(i + 1, SEGMENT - 1)];
                     if (place == 0) {
                         if (!take()) break;
                         to = dst;
                         bar = lead_bar<PAIR>(full0 + 8 * stage);
                     }
-                    const int4 step = ctl.steps[table][i];
-                    const int u_n = __shfl_sync(0xffffffffu, (step.w >> 16) / CTAS, 0);
-                    mbar_expect_more_on(full0 + 8 * stage, (uint32_t)(v_rows * U_RANKS * 2 + u_n * U_BYTES) * CTAS, on_lead);
-                    if (v_rows == VT) {
-                        tma_3d<PAIR>(to, &maps.b[0], 0, step.x + v0 / 4, step.y, bar, on);
+                    if (v_side) {
+                        mbar_expect_more_on(full0 + 8 * stage, (uint32_t)(v_rows * U_RANKS * 2 * CTAS), on_lead);
+                        copy_b(step.x + v0 / 4, step.y, to, bar);
                     } else {
+                        const int u_n = __shfl_sync(0xffffffffu, (step.w >> 16) / CTAS, 0);
+                        mbar_expect_more_on(full0 + 8 * stage, (uint32_t)(u_n * U_BYTES * CTAS), on_lead);
 #pragma unroll 1
-                        for (int m = 1, r = 0; m < 4; m++) {
-                            if (v_rows & VT >> m) {
-                                tma_3d<PAIR>(to + r * 128, &maps.b[m], 0, step.x + v0 / 4 + r, step.y, bar, on);
-                                r += (VT >> m) / 4;
-                            }
-                        }
+                        for (int r = 0; r < u_n; r += a.u_box)  // two rows of u to 128 bytes
+                            tma_2d<PAIR>(to + B_BYTES + r * U_BYTES, &maps.u, 0, (step.z + half * u_n + r) / 2, bar, on);
                     }
-#pragma unroll 1
-                    for (int r = 0; r < u_n; r += a.u_box)  // two rows of u to 128 bytes
-                        tma_2d<PAIR>(to + B_BYTES + r * U_BYTES, &maps.u, 0, (step.z + half * u_n + r) / 2, bar, on);
                     to += (uint32_t)a.pack_bytes;
                     if (++place == a.pack || i == n - 1) {
                         mbar_arrive_on(full0 + 8 * stage, on_lead);
                         place = 0;
                         advance();
                     }
+                    step = next;
                 }
                 if (ok) mbar_arrive_on(smem_u32(&ctl.steps_empty[table]), on);
             }
@@ -524,13 +531,15 @@ __global__ void __launch_bounds__(HEAD_NT, 1) head_rows_kernel(const HeadArgs a,
                     more = __shfl_sync(0xffffffffu, ctl.more[table], 0);
                     int place = 0;
                     uint32_t at = 0;
+                    int window = ctl.steps[table][0].w;
 #pragma unroll 1
                     for (int i = 0; i < n; i++) {
+                        const int next = ctl.steps[table][min(i + 1, SEGMENT - 1)].w;
                         if (place == 0) {
                             if (!take()) break;
                             at = src;
                         }
-                        const int window = __shfl_sync(0xffffffffu, ctl.steps[table][i].w, 0);
+                        window = __shfl_sync(0xffffffffu, window, 0);
                         const uint32_t d = acc + (uint32_t)(window & 0xffff), n_shape = shape_bf16<PAIR>(window >> 16);
                         const uint32_t b_lo = operand_lo(BLOCKS_LO, at), u_lo = operand_lo(BLOCKS_LO, at + B_BYTES);
                         mma<PAIR, false>(d, b_lo, B_BLOCKS_HI, u_lo, U_BLOCKS_HI, n_shape, true, on);             // leading parts
@@ -540,6 +549,7 @@ __global__ void __launch_bounds__(HEAD_NT, 1) head_rows_kernel(const HeadArgs a,
                             place = 0;
                             advance();
                         }
+                        window = next;
                     }
                     if (ok) mbar_arrive_on(smem_u32(&ctl.steps_empty[table]), on);
                 }
