@@ -52,6 +52,8 @@ extern "C" {
  *   out_scale    [rows][scale_stride] float32, given exactly when out_dtype is MANTLE_DTYPE_E4M3;
  *                1 value a row for scale_group 0, ceil(hidden / scale_group) else
  *
+ *   status       optional: as in MantleHeadBatch
+ *
  * Strides are in elements.  residual_out may be x or residual itself, out may be x itself (same type and
  * stride); apart from that no output may overlap an input or another output.  hidden, strides and
  * addresses may be odd: rows that do not start on 16 bytes take element-wise loads.
@@ -63,6 +65,7 @@ typedef struct MantleNormBatch {
     const void* weight;
     void* out;
     float* out_scale;
+    int32_t* status;
     int64_t x_stride;
     int64_t residual_stride;
     int64_t residual_out_stride;

@@ -73,7 +73,7 @@ const char* norm_fault(const MantleNormBatch* b) {
         return "norm: eps must be finite and not negative, weight_offset finite";
     const size_t e = size_of(b->dtype);
     if (!on(b->x, e) || !on(b->residual, e) || !on(b->residual_out, e) || !on(b->out, size_of(b->out_dtype)) ||
-        !on(b->out_scale, 4) || (b->weight && !on(b->weight, size_of(b->weight_dtype))))
+        !on(b->out_scale, 4) || !on(b->status, 4) || (b->weight && !on(b->weight, size_of(b->weight_dtype))))
         return "norm: an address is not a multiple of its element size";
     return nullptr;
 }
@@ -282,6 +282,7 @@ extern "C" int mantleCudaNormRows(const MantleNormBatch* b, mantleCudaStream_t s
     a.weight_f32 = b->weight_dtype == MANTLE_DTYPE_F32;
     a.eps = b->eps;
     a.offset = b->weight_offset;
+    a.status = b->status;
     const bool quant = b->out_dtype == MANTLE_DTYPE_E4M3;
     const int64_t e = (int64_t)size_of(b->dtype);
     auto rows_on_16 = [&](const void* p, int64_t stride) { return !p || (on(p, 16) && stride * e % 16 == 0); };

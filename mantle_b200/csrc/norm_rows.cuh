@@ -23,6 +23,7 @@ struct NormArgs {
     int rows, hidden, group;
     int weight_f32;
     float eps, offset;
+    int* status;
 };
 
 constexpr int NORM_NT = 512;  // threads of a row at most; times 8 eights MANTLE_NORM_MAX_HIDDEN columns
@@ -54,11 +55,11 @@ __device__ __forceinline__ uint32_t pack_e4m3(float lo, float hi) {
 __device__ __forceinline__ float bf16_lo(uint32_t u) { return __uint_as_float(u << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t u) { return __uint_as_float(u & 0xffff0000u); }
 
-__device__ __forceinline__ void load8(const bf16_raw* p, float v[8]) {
-    const uint4 u = *reinterpret_cast<const uint4*>(p);
+__device__ __forceinline__ void eight_of(const uint4& u, float v[8]) {
     v[0] = bf16_lo(u.x), v[1] = bf16_hi(u.x), v[2] = bf16_lo(u.y), v[3] = bf16_hi(u.y);
     v[4] = bf16_lo(u.z), v[5] = bf16_hi(u.z), v[6] = bf16_lo(u.w), v[7] = bf16_hi(u.w);
 }
+__device__ __forceinline__ void load8(const bf16_raw* p, float v[8]) { eight_of(*reinterpret_cast<const uint4*>(p), v); }
 __device__ __forceinline__ void load8(const float* p, float v[8]) {
     const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
     v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
@@ -97,99 +98,84 @@ __device__ __forceinline__ float row_reduce(float v, float* part) {
     return v;
 }
 
-// T: float or bf16_raw.  QUANT: out in e4m3.  VPT: eights of columns a thread holds.  VEC: every row of every
-// operand starts on 16 bytes and hidden is a multiple of 8; a thread's eights are then contiguous, else it
-// holds single columns a row's threads apart.
-template <typename T, bool QUANT, int VPT, bool VEC, bool WARP_ROW>
-__global__ void __launch_bounds__(WARP_ROW ? 128 : NORM_NT) norm_rows_kernel(const NormArgs a) {
-    __shared__ float part[2][32];
-    __shared__ uint32_t group_max[VEC || !QUANT ? 1 : MANTLE_NORM_MAX_HIDDEN / MANTLE_NORM_GROUP];
-    const int tpr = WARP_ROW ? 32 : (int)blockDim.x;
-    const int t = WARP_ROW ? (int)(threadIdx.x & 31) : (int)threadIdx.x;
-    const long long row = WARP_ROW ? (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
-    if (WARP_ROW && row >= a.rows) return;
-    const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
-    const T* res = a.residual ? static_cast<const T*>(a.residual) + row * a.residual_stride : nullptr;
-    T* res_out = a.residual_out ? static_cast<T*>(a.residual_out) + row * a.residual_out_stride : nullptr;
+// What a thread holds of a row: VPT times eight columns.  VEC: every row of every operand starts on 16 bytes and hidden
+// is a multiple of 8; the eights are then contiguous, else single columns, the row's threads apart.
+template <int VPT, bool VEC>
+struct NormCols {
+    int t, tpr, hidden;
+    __device__ __forceinline__ int at(int j, int e) const { return VEC ? (j * tpr + t) * 8 + e : (j * 8 + e) * tpr + t; }
+    __device__ __forceinline__ bool has(int j, int e = 0) const { return at(j, e) < hidden; }
+};
 
-    float s[VPT][8];
-    // column of element e of eight j
-    auto col = [&](int j, int e) { return VEC ? (j * tpr + t) * 8 + e : (j * 8 + e) * tpr + t; };
-    float sum = 0.0f;
-    if constexpr (VEC) {
+// The row's factors, asked for before the sum of squares is known so that they arrive meanwhile, as far as registers
+// reach.  bfloat16 weights of whole eights stay packed until they are used.
+template <int VPT, bool VEC>
+struct NormWeight {
+    static constexpr bool EARLY = VPT <= (VEC ? 4 : 2);
+    uint4 raw[VEC && EARLY ? VPT : 1];
+    float one[!VEC && EARLY ? VPT : 1][8];
+    __device__ __forceinline__ void load(const NormArgs& a, const NormCols<VPT, VEC>& c) {
+        if (!EARLY) return;
 #pragma unroll
         for (int j = 0; j < VPT; j++) {
-            if (col(j, 0) < a.hidden) {
-                load8(x + col(j, 0), s[j]);
+            if constexpr (!EARLY) {
+            } else if constexpr (VEC) {
+                if (a.weight && !a.weight_f32 && c.has(j)) raw[j] = *reinterpret_cast<const uint4*>(static_cast<const bf16_raw*>(a.weight) + c.at(j, 0));
             } else {
 #pragma unroll
-                for (int e = 0; e < 8; e++) s[j][e] = 0.0f;
-            }
-        }
-        if (res) {
-#pragma unroll
-            for (int j = 0; j < VPT; j++) {
-                if (col(j, 0) >= a.hidden) continue;
-                float r[8];
-                load8(res + col(j, 0), r);
-#pragma unroll
-                for (int e = 0; e < 8; e++) s[j][e] += r[e];
-            }
-        }
-        if (res_out) {
-#pragma unroll
-            for (int j = 0; j < VPT; j++)
-                if (col(j, 0) < a.hidden) store8(res_out + col(j, 0), s[j]);
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < VPT; j++) {
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const int c = col(j, e);
-                s[j][e] = 0.0f;
-                if (c < a.hidden) {
-                    s[j][e] = load1(x + c);
-                    if (res) s[j][e] += load1(res + c);
-                    if (res_out) store1(res_out + c, s[j][e]);
-                }
+                for (int e = 0; e < 8; e++) one[j][e] = one_of(a, c, j, e);
             }
         }
     }
+    __device__ __forceinline__ float one_of(const NormArgs& a, const NormCols<VPT, VEC>& c, int j, int e) const {
+        if (!a.weight || !c.has(j, e)) return 1.0f;
+        return a.weight_f32 ? load1(static_cast<const float*>(a.weight) + c.at(j, e))
+                            : load1(static_cast<const bf16_raw*>(a.weight) + c.at(j, e));
+    }
+    __device__ __forceinline__ void get(const NormArgs& a, const NormCols<VPT, VEC>& c, int j, float w[8]) const {
+        if constexpr (VEC) {
+            if (!a.weight || !c.has(j)) {
+#pragma unroll
+                for (int e = 0; e < 8; e++) w[e] = 1.0f;
+            } else if (a.weight_f32) {
+                load8(static_cast<const float*>(a.weight) + c.at(j, 0), w);
+            } else if constexpr (EARLY) {
+                eight_of(raw[j], w);
+            } else {
+                load8(static_cast<const bf16_raw*>(a.weight) + c.at(j, 0), w);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                if constexpr (EARLY) w[e] = one[j][e];
+                else w[e] = one_of(a, c, j, e);
+            }
+        }
+    }
+};
+
+// From the row's s, in registers, to its outputs: the sum of squares, y in the place of s, the scales, the stores.
+// `after_sum` runs once every thread of the row holds its part of s.
+template <typename T, bool QUANT, int VPT, bool VEC, bool WARP_ROW, class F>
+__device__ __forceinline__ void norm_finish(const NormArgs& a, long long row, const NormCols<VPT, VEC>& c, float s[VPT][8],
+                                            const NormWeight<VPT, VEC>& weight, float (*part)[32], uint32_t* group_max, F after_sum) {
+    float sum = 0.0f;
 #pragma unroll
     for (int j = 0; j < VPT; j++) {
 #pragma unroll
         for (int e = 0; e < 8; e++) sum = __fmaf_rn(s[j][e], s[j][e], sum);
     }
     sum = row_reduce<WARP_ROW, false>(sum, part[0]);
+    after_sum();
     const float rstd = __frsqrt_rn(__fadd_rn(__fdiv_rn(sum, (float)a.hidden), a.eps));
-
-    // y in the place of s
 #pragma unroll
     for (int j = 0; j < VPT; j++) {
         float w[8];
-#pragma unroll
-        for (int e = 0; e < 8; e++) w[e] = 1.0f;
-        if (a.weight) {
-            if constexpr (VEC) {
-                if (col(j, 0) < a.hidden) {
-                    if (a.weight_f32) load8(static_cast<const float*>(a.weight) + col(j, 0), w);
-                    else load8(static_cast<const bf16_raw*>(a.weight) + col(j, 0), w);
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const int c = col(j, e);
-                    if (c < a.hidden)
-                        w[e] = a.weight_f32 ? load1(static_cast<const float*>(a.weight) + c)
-                                            : load1(static_cast<const bf16_raw*>(a.weight) + c);
-                }
-            }
-        }
+        weight.get(a, c, j, w);
 #pragma unroll
         for (int e = 0; e < 8; e++) {
             const float y = (s[j][e] * rstd) * (w[e] + a.offset);
-            s[j][e] = col(j, e) < a.hidden ? y : 0.0f;  // past the row: nothing that a maximum would see
+            s[j][e] = c.has(j, e) ? y : 0.0f;  // past the row: nothing that a maximum would see
         }
     }
 
@@ -198,114 +184,274 @@ __global__ void __launch_bounds__(WARP_ROW ? 128 : NORM_NT) norm_rows_kernel(con
 #pragma unroll
         for (int j = 0; j < VPT; j++) {
             if constexpr (VEC) {
-                if (col(j, 0) < a.hidden) store8(out + col(j, 0), s[j]);
+                if (c.has(j)) store8(out + c.at(j, 0), s[j]);
             } else {
 #pragma unroll
                 for (int e = 0; e < 8; e++)
-                    if (col(j, e) < a.hidden) store1(out + col(j, e), s[j][e]);
+                    if (c.has(j, e)) store1(out + c.at(j, e), s[j][e]);
             }
-        }
-        return;
-    }
-
-    uint8_t* out = static_cast<uint8_t*>(a.out) + row * a.out_stride;
-    float* scales = a.scale + row * a.scale_stride;
-    // Multiplying by the scale's reciprocal differs from dividing in the last float32 bit only: two rounding
-    // errors of 2^-24 before one of 2^-4.
-    if (a.group == 0) {
-        float m = 0.0f;
-#pragma unroll
-        for (int j = 0; j < VPT; j++) {
-#pragma unroll
-            for (int e = 0; e < 8; e++) m = max_nan(m, fabsf(s[j][e]));
-        }
-        m = row_reduce<WARP_ROW, true>(m, part[1]);
-        const float scale = max_nan(__fdiv_rn(m, E4M3_MAX), E4M3_SCALE_MIN), inv = __frcp_rn(scale);
-        if (t == 0) scales[0] = scale;
-#pragma unroll
-        for (int j = 0; j < VPT; j++) {
-#pragma unroll
-            for (int e = 0; e < 8; e++) s[j][e] *= inv;
-        }
-    } else if constexpr (VEC) {
-        // sixteen neighbouring threads hold the 128 columns of a group
-#pragma unroll
-        for (int j = 0; j < VPT; j++) {
-            float m = 0.0f;
-#pragma unroll
-            for (int e = 0; e < 8; e++) m = max_nan(m, fabsf(s[j][e]));
-#pragma unroll
-            for (int o = 8; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-            const float scale = max_nan(__fdiv_rn(m, E4M3_MAX), E4M3_SCALE_MIN), inv = __frcp_rn(scale);
-            if (t % 16 == 0 && col(j, 0) < a.hidden) scales[col(j, 0) / MANTLE_NORM_GROUP] = scale;
-#pragma unroll
-            for (int e = 0; e < 8; e++) s[j][e] *= inv;
         }
     } else {
-        // the bits of non-negative floats order like integers, NaN above all
-        const int groups = (a.hidden + MANTLE_NORM_GROUP - 1) / MANTLE_NORM_GROUP;
-        for (int g = threadIdx.x; g < groups; g += blockDim.x) group_max[g] = 0;
-        __syncthreads();
+        uint8_t* out = static_cast<uint8_t*>(a.out) + row * a.out_stride;
+        float* scales = a.scale + row * a.scale_stride;
+        // Multiplying by the scale's reciprocal differs from dividing in the last float32 bit only: two rounding
+        // errors of 2^-24 before one of 2^-4.
+        if (a.group == 0) {
+            float m = 0.0f;
 #pragma unroll
-        for (int j = 0; j < VPT; j++) {
+            for (int j = 0; j < VPT; j++) {
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(s[j][e])));
-                // a warp's 32 columns start on a multiple of 32: one group
-                if ((threadIdx.x & 31) == 0 && col(j, e) < a.hidden) atomicMax(&group_max[col(j, e) / MANTLE_NORM_GROUP], m);
+                for (int e = 0; e < 8; e++) m = max_nan(m, fabsf(s[j][e]));
             }
-        }
-        __syncthreads();
-        for (int g = threadIdx.x; g < groups; g += blockDim.x)
-            scales[g] = max_nan(__fdiv_rn(__uint_as_float(group_max[g]), E4M3_MAX), E4M3_SCALE_MIN);
+            m = row_reduce<WARP_ROW, true>(m, part[1]);
+            const float scale = max_nan(__fdiv_rn(m, E4M3_MAX), E4M3_SCALE_MIN), inv = __frcp_rn(scale);
+            if (c.t == 0) scales[0] = scale;
 #pragma unroll
-        for (int j = 0; j < VPT; j++) {
+            for (int j = 0; j < VPT; j++) {
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                if (col(j, e) >= a.hidden) continue;
-                const float m = __uint_as_float(group_max[col(j, e) / MANTLE_NORM_GROUP]);
-                s[j][e] *= __frcp_rn(max_nan(__fdiv_rn(m, E4M3_MAX), E4M3_SCALE_MIN));
+                for (int e = 0; e < 8; e++) s[j][e] *= inv;
             }
-        }
-    }
+        } else if constexpr (VEC) {
+            // sixteen neighbouring threads hold the 128 columns of a group
 #pragma unroll
-    for (int j = 0; j < VPT; j++) {
-        if constexpr (VEC) {
-            if (col(j, 0) < a.hidden)
-                *reinterpret_cast<uint2*>(out + col(j, 0)) =
-                    make_uint2(pack_e4m3(s[j][0], s[j][1]) | pack_e4m3(s[j][2], s[j][3]) << 16,
-                               pack_e4m3(s[j][4], s[j][5]) | pack_e4m3(s[j][6], s[j][7]) << 16);
+            for (int j = 0; j < VPT; j++) {
+                float m = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 8; e++) m = max_nan(m, fabsf(s[j][e]));
+#pragma unroll
+                for (int o = 8; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+                const float scale = max_nan(__fdiv_rn(m, E4M3_MAX), E4M3_SCALE_MIN), inv = __frcp_rn(scale);
+                if (c.t % 16 == 0 && c.has(j)) scales[c.at(j, 0) / MANTLE_NORM_GROUP] = scale;
+#pragma unroll
+                for (int e = 0; e < 8; e++) s[j][e] *= inv;
+            }
         } else {
+            // the bits of non-negative floats order like integers, NaN above all
+            const int groups = (a.hidden + MANTLE_NORM_GROUP - 1) / MANTLE_NORM_GROUP;
+            for (int g = threadIdx.x; g < groups; g += blockDim.x) group_max[g] = 0;
+            __syncthreads();
 #pragma unroll
-            for (int e = 0; e < 8; e++)
-                if (col(j, e) < a.hidden) out[col(j, e)] = (uint8_t)pack_e4m3(s[j][e], 0.0f);
+            for (int j = 0; j < VPT; j++) {
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(s[j][e])));
+                    // a warp's 32 columns start on a multiple of 32: one group
+                    if ((threadIdx.x & 31) == 0 && c.has(j, e)) atomicMax(&group_max[c.at(j, e) / MANTLE_NORM_GROUP], m);
+                }
+            }
+            __syncthreads();
+            for (int g = threadIdx.x; g < groups; g += blockDim.x)
+                scales[g] = max_nan(__fdiv_rn(__uint_as_float(group_max[g]), E4M3_MAX), E4M3_SCALE_MIN);
+#pragma unroll
+            for (int j = 0; j < VPT; j++) {
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    if (!c.has(j, e)) continue;
+                    const float m = __uint_as_float(group_max[c.at(j, e) / MANTLE_NORM_GROUP]);
+                    s[j][e] *= __frcp_rn(max_nan(__fdiv_rn(m, E4M3_MAX), E4M3_SCALE_MIN));
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < VPT; j++) {
+            if constexpr (VEC) {
+                if (c.has(j))
+                    *reinterpret_cast<uint2*>(out + c.at(j, 0)) =
+                        make_uint2(pack_e4m3(s[j][0], s[j][1]) | pack_e4m3(s[j][2], s[j][3]) << 16,
+                                   pack_e4m3(s[j][4], s[j][5]) | pack_e4m3(s[j][6], s[j][7]) << 16);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    if (c.has(j, e)) out[c.at(j, e)] = (uint8_t)pack_e4m3(s[j][e], 0.0f);
+            }
         }
     }
 }
 
-template <typename T, bool QUANT, int VPT, bool VEC>
-int launch_norm_vpt(const NormArgs& a, int threads, cudaStream_t stream) {
-    norm_rows_kernel<T, QUANT, VPT, VEC, false><<<a.rows, threads, 0, stream>>>(a);
-    return (int)cudaGetLastError();
+// One row for a warp or a CTA.
+template <typename T, bool QUANT, int VPT, bool VEC, bool WARP_ROW>
+__global__ void __launch_bounds__(WARP_ROW ? 128 : NORM_NT) norm_rows_kernel(const NormArgs a) {
+    __shared__ float part[2][32];
+    __shared__ uint32_t group_max[VEC || !QUANT ? 1 : MANTLE_NORM_MAX_HIDDEN / MANTLE_NORM_GROUP];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const long long row = WARP_ROW ? (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
+    if (WARP_ROW && row >= a.rows) return;
+    const NormCols<VPT, VEC> c = {WARP_ROW ? (int)(threadIdx.x & 31) : (int)threadIdx.x, WARP_ROW ? 32 : (int)blockDim.x, a.hidden};
+    const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
+    const T* res = a.residual ? static_cast<const T*>(a.residual) + row * a.residual_stride : nullptr;
+    T* res_out = a.residual_out ? static_cast<T*>(a.residual_out) + row * a.residual_out_stride : nullptr;
+    constexpr bool EARLY = NormWeight<VPT, VEC>::EARLY;
+    float s[VPT][8], r[EARLY ? VPT : 1][8];
+    // all loads before the first use, as far as registers reach
+#pragma unroll
+    for (int j = 0; j < VPT; j++) {
+        if constexpr (VEC) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) s[j][e] = 0.0f;
+            if (c.has(j)) load8(x + c.at(j, 0), s[j]);
+            if (EARLY && res && c.has(j)) load8(res + c.at(j, 0), r[EARLY ? j : 0]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                s[j][e] = c.has(j, e) ? load1(x + c.at(j, e)) : 0.0f;
+                if (EARLY && res) r[EARLY ? j : 0][e] = c.has(j, e) ? load1(res + c.at(j, e)) : 0.0f;
+            }
+        }
+    }
+    NormWeight<VPT, VEC> weight;
+    weight.load(a, c);
+    if (res) {
+#pragma unroll
+        for (int j = 0; j < VPT; j++) {
+            if constexpr (VEC) {
+                if (!c.has(j)) continue;
+                if (!EARLY) load8(res + c.at(j, 0), r[0]);
+            } else if (!EARLY) {
+#pragma unroll
+                for (int e = 0; e < 8; e++) r[0][e] = c.has(j, e) ? load1(res + c.at(j, e)) : 0.0f;
+            }
+#pragma unroll
+            for (int e = 0; e < 8; e++) s[j][e] += r[EARLY ? j : 0][e];
+            if (!res_out) continue;
+            if constexpr (VEC) {
+                store8(res_out + c.at(j, 0), s[j]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    if (c.has(j, e)) store1(res_out + c.at(j, e), s[j][e]);
+            }
+        }
+    }
+    norm_finish<T, QUANT, VPT, VEC, WARP_ROW>(a, row, c, s, weight, part, group_max, [] {});
+}
+
+// Many long rows: CTAs that stay, each with a ring of two rows of x and residual in shared memory that bulk copies fill
+// ahead.  In registers alone an SM holds no more bytes in flight than its threads have room for beside the row they
+// work on, and none at all between a CTA's end and the next one's first load (16 384 x 8192 bfloat16 with residual, to
+// 8 bits: 243 us so, TODO us here).
+constexpr int NORM_RING = 2;
+constexpr int NORM_STREAM_NT = 256;
+
+template <typename T, bool QUANT, int VPT>
+__global__ void __launch_bounds__(NORM_STREAM_NT) norm_stream_kernel(const NormArgs a) {
+    extern __shared__ __align__(128) char ring[];  // [NORM_RING][x, residual][row_bytes]
+    __shared__ float part[2][2][32];               // a row's, and the next one's
+    __shared__ uint64_t full[NORM_RING];
+    const uint32_t row_bytes = (uint32_t)a.hidden * sizeof(T), operands = a.residual ? 2 : 1;
+    const NormCols<VPT, true> c = {(int)threadIdx.x, (int)blockDim.x, a.hidden};
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < NORM_RING; i++) mbar_init(&full[i], 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    auto fetch = [&](long long row, int slot) {  // one thread
+        const uint32_t bar = smem_u32(&full[slot]), dst = smem_u32(ring) + (uint32_t)slot * operands * row_bytes;
+        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(operands * row_bytes) : "memory");
+        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                     ::"r"(dst), "l"(static_cast<const T*>(a.x) + row * a.x_stride), "r"(row_bytes), "r"(bar) : "memory");
+        if (a.residual)
+            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                         ::"r"(dst + row_bytes), "l"(static_cast<const T*>(a.residual) + row * a.residual_stride), "r"(row_bytes), "r"(bar) : "memory");
+    };
+    NormWeight<VPT, true> weight;
+    weight.load(a, c);
+    if (threadIdx.x == 0)
+        for (int i = 0; i < NORM_RING; i++)
+            if ((long long)blockIdx.x + (long long)i * gridDim.x < a.rows) fetch((long long)blockIdx.x + (long long)i * gridDim.x, i);
+    int n = 0;
+    for (long long row = blockIdx.x; row < a.rows; row += gridDim.x, n++) {
+        const int slot = n % NORM_RING;
+        // a copy that does not come in two seconds: the CTA says so and gives up together, when its other copies are in
+        if (!__syncthreads_and(mbar_wait(&full[slot], (uint32_t)(n / NORM_RING) & 1))) {
+            if (threadIdx.x == 0) {
+                if (a.status) atomicOr(a.status, MANTLE_SAMPLE_STATUS_TIMEOUT);
+                for (int i = 1; i < NORM_RING && row + (long long)i * gridDim.x < a.rows; i++)
+                    mbar_wait(&full[(n + i) % NORM_RING], (uint32_t)((n + i) / NORM_RING) & 1, 100000000ull);
+            }
+            return;
+        }
+        const T* x = reinterpret_cast<const T*>(ring + (size_t)slot * operands * row_bytes);
+        float s[VPT][8];
+#pragma unroll
+        for (int j = 0; j < VPT; j++) {
+            if (c.has(j)) {
+                load8(x + c.at(j, 0), s[j]);
+                if (a.residual) {
+                    float r[8];
+                    load8(x + a.hidden + c.at(j, 0), r);
+#pragma unroll
+                    for (int e = 0; e < 8; e++) s[j][e] += r[e];
+                    if (a.residual_out) store8(static_cast<T*>(a.residual_out) + row * a.residual_out_stride + c.at(j, 0), s[j]);
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; e++) s[j][e] = 0.0f;
+            }
+        }
+        norm_finish<T, QUANT, VPT, true, false>(a, row, c, s, weight, part[n & 1], nullptr, [&] {
+            // behind the sum's barrier every thread has taken its part of the slot
+            const long long ahead = row + (long long)NORM_RING * gridDim.x;
+            if (threadIdx.x == 0 && ahead < a.rows) fetch(ahead, slot);
+        });
+    }
+}
+
+// Every norm kernel waits for what is in front of it by itself, so that its launch overlaps that kernel's end.
+int launch_norm_kernel(void (*kern)(NormArgs), const NormArgs& a, int grid, int threads, size_t smem, cudaStream_t stream) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return (int)cudaLaunchKernelEx(&cfg, kern, a);
+}
+
+template <typename T, bool QUANT, int VPT>
+int launch_norm_stream(const NormArgs& a, int per_sm, size_t smem, cudaStream_t stream) {
+    static std::atomic<int> granted[kMaxDevices];
+    const auto kern = norm_stream_kernel<T, QUANT, VPT>;
+    const int rc = ensure_smem(kern, smem, granted);
+    if (rc) return rc;
+    return launch_norm_kernel(kern, a, std::min(a.rows, device_sms() * per_sm), NORM_STREAM_NT, smem, stream);
 }
 
 template <typename T, bool QUANT, bool VEC>
 int launch_norm_as(const NormArgs& a, cudaStream_t stream) {
     const int eights = (a.hidden + 7) / 8;
-    // rows of a warp go four to a CTA; not so where element-wise rows need the CTA's group maxima
-    if (eights <= 32 && (VEC || !QUANT)) {
-        norm_rows_kernel<T, QUANT, 1, VEC, true><<<(a.rows + 3) / 4, 128, 0, stream>>>(a);
-        return (int)cudaGetLastError();
+    const bool many = a.rows > 2 * device_sms();
+    // A warp a row, four to a CTA: short rows, and rows of up to 1024 columns where there are many.  (Not where
+    // element-wise rows need the CTA's group maxima.)
+    if (VEC || !QUANT) {
+        const int grid = (a.rows + 3) / 4;
+        if (eights <= 32) return launch_norm_kernel(norm_rows_kernel<T, QUANT, 1, VEC, true>, a, grid, 128, 0, stream);
+        if (many && eights <= 64) return launch_norm_kernel(norm_rows_kernel<T, QUANT, 2, VEC, true>, a, grid, 128, 0, stream);
+        if (many && eights <= 128) return launch_norm_kernel(norm_rows_kernel<T, QUANT, 4, VEC, true>, a, grid, 128, 0, stream);
     }
-    // Few rows: as few eights a thread as 512 threads allow, the shortest path through the kernel.  Many rows: up to
-    // four, more bytes in flight for the same threads.
+    if constexpr (VEC) {
+        // The ring: where an SM gets several rows, and a row is worth a bulk copy.  Two CTAs of it have to fit.
+        const size_t smem = (size_t)NORM_RING * (a.residual ? 2 : 1) * (size_t)a.hidden * sizeof(T);
+        const int per_sm = (int)std::min<size_t>(6, (size_t)device_info().per_sm / (smem + 2048));
+        if (a.rows >= 16 * device_sms() && eights >= 256 && eights <= 4 * NORM_STREAM_NT && per_sm >= 2) {
+            if (eights <= NORM_STREAM_NT) return launch_norm_stream<T, QUANT, 1>(a, per_sm, smem, stream);
+            if (eights <= 2 * NORM_STREAM_NT) return launch_norm_stream<T, QUANT, 2>(a, per_sm, smem, stream);
+            return launch_norm_stream<T, QUANT, 4>(a, per_sm, smem, stream);
+        }
+    }
+    // A CTA a row.  Few rows: as few eights a thread as 512 threads allow, the shortest path through the kernel.  Many
+    // rows: up to four, more bytes in flight for the same threads.
     int vpt = 1;
-    while (eights > vpt * NORM_NT || (vpt < 4 && a.rows > 2 * device_sms() && eights >= vpt * 128)) vpt *= 2;
+    while (eights > vpt * NORM_NT || (vpt < 4 && many && eights >= vpt * 128)) vpt *= 2;
     const int threads = ((eights + vpt - 1) / vpt + 31) / 32 * 32;
-    if (vpt == 1) return launch_norm_vpt<T, QUANT, 1, VEC>(a, threads, stream);
-    if (vpt == 2) return launch_norm_vpt<T, QUANT, 2, VEC>(a, threads, stream);
-    if (vpt == 4) return launch_norm_vpt<T, QUANT, 4, VEC>(a, threads, stream);
-    return launch_norm_vpt<T, QUANT, 8, VEC>(a, threads, stream);
+    if (vpt == 1) return launch_norm_kernel(norm_rows_kernel<T, QUANT, 1, VEC, false>, a, a.rows, threads, 0, stream);
+    if (vpt == 2) return launch_norm_kernel(norm_rows_kernel<T, QUANT, 2, VEC, false>, a, a.rows, threads, 0, stream);
+    if (vpt == 4) return launch_norm_kernel(norm_rows_kernel<T, QUANT, 4, VEC, false>, a, a.rows, threads, 0, stream);
+    return launch_norm_kernel(norm_rows_kernel<T, QUANT, 8, VEC, false>, a, a.rows, threads, 0, stream);
 }
 
 template <typename T>

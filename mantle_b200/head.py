@@ -20,6 +20,7 @@ import torch
 
 from . import native
 
+_raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 _DTYPES = {torch.float32: native.DTYPE_F32, torch.bfloat16: native.DTYPE_BF16, torch.float8_e4m3fn: native.DTYPE_E4M3}
 
 
@@ -68,24 +69,21 @@ def _same(a, b):
 
 
 class _Plan:
-    def _stream(self, stream):
-        # the stream that is current on the plan's device, whatever device is current
-        return torch._C._cuda_getCurrentRawStream(self._index) if stream is None else stream.cuda_stream
-
     def _bind(self, device):
         self.device = device
         self._index = device.index
         self.lib = native.load()
 
-    def _launch(self, fn, where, args, stream):
-        s = self._stream(stream)
-        if torch._C._cuda_getDevice() == self._index:
-            rc = fn(*args, s)
+    def _queue(self, stream):
+        # the stream that is current on the plan's device, whatever device is current
+        s = _raw_stream(self._index) if stream is None else stream.cuda_stream
+        if _current_device() == self._index:
+            rc = self._fn(*self._args, s)
         else:
             with torch.cuda.device(self._index):
-                rc = fn(*args, s)
+                rc = self._fn(*self._args, s)
         if rc:
-            _check(self.lib, rc, where)
+            _check(self.lib, rc, self._name)
 
 
 class NormOutputs:
@@ -150,19 +148,21 @@ class NormPlan(_Plan):
                 in_place = (n, m) in (("out", "x"), ("residual_out", "x"), ("residual_out", "residual")) and _same(t, u)
                 if _overlap(t, u) and not in_place:
                     raise ValueError("%s overlaps %s" % (n, m))
+        self.status = torch.zeros(1, dtype=torch.int32, device=dev)
+        b.status = self.status.data_ptr()
         self.rows, self.hidden = rows, hidden
         self.out, self.scales, self.residual_out = out, scales, residual_out
         self.keep = [x, weight, residual]
         self.batch = b
         self._args = (C.byref(b),)
-        self._fn = self.lib.mantleCudaNormRows
+        self._fn, self._name = self.lib.mantleCudaNormRows, "mantleCudaNormRows"
         o = NormOutputs()
         o.out, o.scales, o.residual_out = out, scales, residual_out
         self._outputs = o
 
     def launch(self, stream=None):
         """Queues the norm on `stream` (default: the device's current stream).  Does not synchronise."""
-        self._launch(self._fn, "mantleCudaNormRows", self._args, stream)
+        self._queue(stream)
         return self._outputs
 
 
@@ -306,12 +306,12 @@ class HeadPlan(_Plan):
         self.keep = reads
         self.batch = b
         self._args = (C.byref(b), None if self.workspace is None else self.workspace.data_ptr(), n.value)
-        self._fn = self.lib.mantleCudaHeadRows
+        self._fn, self._name = self.lib.mantleCudaHeadRows, "mantleCudaHeadRows"
 
     def launch(self, stream=None):
         """Queues the projection on `stream` (default: the device's current stream) and returns the logits.
         Does not synchronise."""
-        self._launch(self._fn, "mantleCudaHeadRows", self._args, stream)
+        self._queue(stream)
         return self.out
 
 

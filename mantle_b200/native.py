@@ -86,6 +86,7 @@ class NormBatch(C.Structure):
         ("weight", C.c_void_p),
         ("out", C.c_void_p),
         ("out_scale", C.c_void_p),
+        ("status", C.c_void_p),
         ("x_stride", C.c_int64),
         ("residual_stride", C.c_int64),
         ("residual_out_stride", C.c_int64),

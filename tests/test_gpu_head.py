@@ -79,6 +79,24 @@ def test_norm_strides_offsets_and_weights(quant, group):
             assert bool((rim == 7.0).all())  # nothing beside the rows was written
 
 
+@pytest.mark.parametrize("hidden,dtype", [(2048, BF16), (2056, F32), (4096, BF16), (8192, BF16), (8184, BF16), (4104, F32)])
+def test_norm_of_many_long_rows(hidden, dtype):
+    """Enough rows for the kernel that keeps a ring of them, an odd number for each of its CTAs."""
+    rows = 148 * 17 + 5
+    x, r = (rand(1, rows, hidden) * 2).to(dtype), rand(2, rows, hidden).to(dtype)
+    w = (1 + 0.1 * rand(3, hidden)).to(dtype)
+    for residual, quant, group in itertools.product((False, True), (False, True), (0, 128)):
+        if group and not quant:
+            continue
+        o = check_norm(x, w, r if residual else None, E4M3 if quant else None, group, where=(residual, quant, group))
+    xi, ri = x.clone(), r.clone()
+    got = H.NormPlan(xi, w, residual=ri, out=xi, residual_out=ri)
+    got.launch()
+    want = H.NormPlan(x, w, residual=r).launch()
+    torch.cuda.synchronize()
+    assert torch.equal(xi, want.out) and torch.equal(ri, want.residual_out) and int(got.status.item()) == 0
+
+
 def test_norm_in_place():
     for dtype in (F32, BF16):
         x0, r0 = (rand(1, 50, 1032) * 2).to(dtype), rand(2, 50, 1032).to(dtype)

@@ -25,8 +25,8 @@ def test_library_exports_every_declared_symbol():
 
 
 def test_struct_layouts_match_the_header():
-    assert C.sizeof(native.NormBatch) == 120
-    assert native.NormBatch.x_stride.offset == 48 and native.NormBatch.rows.offset == 88
+    assert C.sizeof(native.NormBatch) == 128
+    assert native.NormBatch.x_stride.offset == 56 and native.NormBatch.rows.offset == 96
     assert C.sizeof(native.HeadBatch) == 152
     assert native.HeadBatch.hidden_stride.offset == 88 and native.HeadBatch.rows.offset == 120
 
