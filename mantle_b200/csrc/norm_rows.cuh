@@ -330,7 +330,7 @@ __global__ void __launch_bounds__(WARP_ROW ? 128 : NORM_NT) norm_rows_kernel(con
 // work on, and none at all between a CTA's end and the next one's first load (16 384 x 8192 bfloat16 with residual, to
 // 8 bits: 243 us so, TODO us here).
 constexpr int NORM_RING = 2;
-constexpr int NORM_STREAM_NT = 256;
+constexpr int NORM_STREAM_NT = 512;  // threads at most
 
 template <typename T, bool QUANT, int VPT>
 __global__ void __launch_bounds__(NORM_STREAM_NT) norm_stream_kernel(const NormArgs a) {
@@ -413,12 +413,12 @@ int launch_norm_kernel(void (*kern)(NormArgs), const NormArgs& a, int grid, int 
 }
 
 template <typename T, bool QUANT, int VPT>
-int launch_norm_stream(const NormArgs& a, int per_sm, size_t smem, cudaStream_t stream) {
+int launch_norm_stream(const NormArgs& a, int threads, int per_sm, size_t smem, cudaStream_t stream) {
     static std::atomic<int> granted[kMaxDevices];
     const auto kern = norm_stream_kernel<T, QUANT, VPT>;
     const int rc = ensure_smem(kern, smem, granted);
     if (rc) return rc;
-    return launch_norm_kernel(kern, a, std::min(a.rows, device_sms() * per_sm), NORM_STREAM_NT, smem, stream);
+    return launch_norm_kernel(kern, a, std::min(a.rows, device_sms() * per_sm), threads, smem, stream);
 }
 
 template <typename T, bool QUANT, bool VEC>
@@ -434,13 +434,14 @@ int launch_norm_as(const NormArgs& a, cudaStream_t stream) {
         if (many && eights <= 128) return launch_norm_kernel(norm_rows_kernel<T, QUANT, 4, VEC, true>, a, grid, 128, 0, stream);
     }
     if constexpr (VEC) {
-        // The ring: where an SM gets several rows, and a row is worth a bulk copy.  Two CTAs of it have to fit.
+        // The ring: where an SM gets several rows, and a row is worth a bulk copy.  Two CTAs of it have to fit.  One
+        // eight a thread up to 2048 columns, two above (8192 columns: 193 us with four and 256 threads, 170 with two).
         const size_t smem = (size_t)NORM_RING * (a.residual ? 2 : 1) * (size_t)a.hidden * sizeof(T);
-        const int per_sm = (int)std::min<size_t>(6, (size_t)device_info().per_sm / (smem + 2048));
-        if (a.rows >= 16 * device_sms() && eights >= 256 && eights <= 4 * NORM_STREAM_NT && per_sm >= 2) {
-            if (eights <= NORM_STREAM_NT) return launch_norm_stream<T, QUANT, 1>(a, per_sm, smem, stream);
-            if (eights <= 2 * NORM_STREAM_NT) return launch_norm_stream<T, QUANT, 2>(a, per_sm, smem, stream);
-            return launch_norm_stream<T, QUANT, 4>(a, per_sm, smem, stream);
+        const int vpt = eights <= 256 ? 1 : 2, threads = ((eights + vpt - 1) / vpt + 31) / 32 * 32;
+        const int per_sm = (int)std::min<size_t>((size_t)(1536 / threads), (size_t)device_info().per_sm / (smem + 2048));
+        if (a.rows >= 16 * device_sms() && eights >= 256 && eights <= 2 * NORM_STREAM_NT && per_sm >= 2) {
+            if (vpt == 1) return launch_norm_stream<T, QUANT, 1>(a, threads, per_sm, smem, stream);
+            return launch_norm_stream<T, QUANT, 2>(a, threads, per_sm, smem, stream);
         }
     }
     // A CTA a row.  Few rows: as few eights a thread as 512 threads allow, the shortest path through the kernel.  Many
