@@ -235,7 +235,7 @@ __device__ __forceinline__ float shrink32(const HeadPrep& p, int adapter, int j0
     const bool both = j0 + 8 < p.rank;  // (the rank may end after eight)
     float d[2][2][4] = {};
     const uint4 none = make_uint4(0, 0, 0, 0);
-#pragma unroll 2
+#pragma unroll 4
     for (int k = warp * 32 + q * 8; k < p.hidden + q * 8; k += SHRINK_WARPS * 32) {  // the same count for a warp's lanes
         const bool in = k < p.hidden;
         uint4 x[4], w[2];
@@ -339,8 +339,8 @@ __global__ void __launch_bounds__(SHRINK_NT) head_shrink_here_kernel(const HeadP
     if (tid < HERE_ROWS) {
         const int id = ids[tid];
         bool first = id >= 0;
-#pragma unroll 8
-        for (int r = 0; r < HERE_ROWS; r += 4) {
+#pragma unroll 4
+        for (int r = 0; r < p.rows; r += 4) {  // (behind the last row: no adapter)
             const int4 v = *reinterpret_cast<const int4*>(ids + r);
             first = first && !(r < tid && v.x == id) && !(r + 1 < tid && v.y == id) && !(r + 2 < tid && v.z == id) && !(r + 3 < tid && v.w == id);
         }
