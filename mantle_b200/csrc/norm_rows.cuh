@@ -151,14 +151,31 @@ struct NormWeight {
                 else w[e] = one_of(a, c, j, e);
             }
         }
+#pragma unroll
+        for (int e = 0; e < 8; e++) w[e] += a.offset;
+    }
+};
+// The same held ready over many rows.
+template <int VPT>
+struct NormWeightHeld {
+    float held[VPT][8];
+    __device__ __forceinline__ void load(const NormArgs& a, const NormCols<VPT, true>& c) {
+        NormWeight<VPT, true> weight;
+        weight.load(a, c);
+#pragma unroll
+        for (int j = 0; j < VPT; j++) weight.get(a, c, j, held[j]);
+    }
+    __device__ __forceinline__ void get(const NormArgs&, const NormCols<VPT, true>&, int j, float w[8]) const {
+#pragma unroll
+        for (int e = 0; e < 8; e++) w[e] = held[j][e];
     }
 };
 
 // From the row's s, in registers, to its outputs: the sum of squares, y in the place of s, the scales, the stores.
 // `after_sum` runs once every thread of the row holds its part of s.
-template <typename T, bool QUANT, int VPT, bool VEC, bool WARP_ROW, class F>
+template <typename T, bool QUANT, int VPT, bool VEC, bool WARP_ROW, class W, class F>
 __device__ __forceinline__ void norm_finish(const NormArgs& a, long long row, const NormCols<VPT, VEC>& c, float s[VPT][8],
-                                            const NormWeight<VPT, VEC>& weight, float (*part)[32], uint32_t* group_max, F after_sum) {
+                                            const W& weight, float (*part)[32], uint32_t* group_max, F after_sum) {
     float sum = 0.0f;
 #pragma unroll
     for (int j = 0; j < VPT; j++) {
@@ -174,8 +191,8 @@ __device__ __forceinline__ void norm_finish(const NormArgs& a, long long row, co
         weight.get(a, c, j, w);
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-            const float y = (s[j][e] * rstd) * (w[e] + a.offset);
-            s[j][e] = c.has(j, e) ? y : 0.0f;  // past the row: nothing that a maximum would see
+            // past the row s is 0 and w is finite: 0, or NaN where the whole row is
+            s[j][e] = (s[j][e] * rstd) * w[e];
         }
     }
 
@@ -325,15 +342,16 @@ __global__ void __launch_bounds__(WARP_ROW ? 128 : NORM_NT) norm_rows_kernel(con
     norm_finish<T, QUANT, VPT, VEC, WARP_ROW>(a, row, c, s, weight, part, group_max, [] {});
 }
 
-// Many long rows: CTAs that stay, each with a ring of two rows of x and residual in shared memory that bulk copies fill
-// ahead.  In registers alone an SM holds no more bytes in flight than its threads have room for beside the row they
+// Many long rows: CTAs that stay, each with a ring of rows of x and residual in shared memory that bulk copies fill ahead.  In registers alone an SM holds no more bytes in flight than its threads have room for beside the row they
 // work on, and none at all between a CTA's end and the next one's first load (16 384 x 8192 bfloat16 with residual, to
-// 8 bits: 243 us so, 170 here).
-constexpr int NORM_RING = 2;
+// 8 bits: 243 us so, 150 here, 97 % of the measured copy bandwidth).  The row's factors stay in registers as they
+// are used: with them packed, and a test for the row's end at every value, instruction issue was the bound (36
+// instructions a value, 170 us).
+constexpr int NORM_RING = 2;          // (four deep measured the same)
 constexpr int NORM_STREAM_NT = 512;  // threads at most
 
 template <typename T, bool QUANT, int VPT>
-__global__ void __launch_bounds__(NORM_STREAM_NT) norm_stream_kernel(const NormArgs a) {
+__global__ void __launch_bounds__(VPT == 1 ? NORM_STREAM_NT / 2 : NORM_STREAM_NT, VPT == 1 ? 6 : 2) norm_stream_kernel(const NormArgs a) {
     extern __shared__ __align__(128) char ring[];  // [NORM_RING][x, residual][row_bytes]
     __shared__ float part[2][2][32];               // a row's, and the next one's
     __shared__ uint64_t full[NORM_RING];
@@ -354,20 +372,20 @@ __global__ void __launch_bounds__(NORM_STREAM_NT) norm_stream_kernel(const NormA
             asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                          ::"r"(dst + row_bytes), "l"(static_cast<const T*>(a.residual) + row * a.residual_stride), "r"(row_bytes), "r"(bar) : "memory");
     };
-    NormWeight<VPT, true> weight;
+    NormWeightHeld<VPT> weight;
     weight.load(a, c);
     if (threadIdx.x == 0)
         for (int i = 0; i < NORM_RING; i++)
             if ((long long)blockIdx.x + (long long)i * gridDim.x < a.rows) fetch((long long)blockIdx.x + (long long)i * gridDim.x, i);
-    int n = 0;
-    for (long long row = blockIdx.x; row < a.rows; row += gridDim.x, n++) {
-        const int slot = n % NORM_RING;
+    int slot = 0, odd = 0;
+    uint32_t turn = 0;  // parity of the slot's phase
+    for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
         // a copy that does not come in two seconds: the CTA says so and gives up together, when its other copies are in
-        if (!__syncthreads_and(mbar_wait(&full[slot], (uint32_t)(n / NORM_RING) & 1))) {
+        if (!__syncthreads_and(mbar_wait(&full[slot], turn))) {
             if (threadIdx.x == 0) {
                 if (a.status) atomicOr(a.status, MANTLE_SAMPLE_STATUS_TIMEOUT);
                 for (int i = 1; i < NORM_RING && row + (long long)i * gridDim.x < a.rows; i++)
-                    mbar_wait(&full[(n + i) % NORM_RING], (uint32_t)((n + i) / NORM_RING) & 1, 100000000ull);
+                    mbar_wait(&full[(slot + i) % NORM_RING], turn ^ (slot + i >= NORM_RING), 100000000ull);
             }
             return;
         }
@@ -389,11 +407,13 @@ __global__ void __launch_bounds__(NORM_STREAM_NT) norm_stream_kernel(const NormA
                 for (int e = 0; e < 8; e++) s[j][e] = 0.0f;
             }
         }
-        norm_finish<T, QUANT, VPT, true, false>(a, row, c, s, weight, part[n & 1], nullptr, [&] {
+        norm_finish<T, QUANT, VPT, true, false>(a, row, c, s, weight, part[odd], nullptr, [&] {
             // behind the sum's barrier every thread has taken its part of the slot
             const long long ahead = row + (long long)NORM_RING * gridDim.x;
             if (threadIdx.x == 0 && ahead < a.rows) fetch(ahead, slot);
         });
+        odd ^= 1;
+        if (++slot == NORM_RING) slot = 0, turn ^= 1;
     }
 }
 
@@ -435,13 +455,14 @@ int launch_norm_as(const NormArgs& a, cudaStream_t stream) {
     }
     if constexpr (VEC) {
         // The ring: where an SM gets several rows, and a row is worth a bulk copy.  Two CTAs of it have to fit.  One
-        // eight a thread up to 2048 columns, two above (8192 columns: 193 us with four and 256 threads, 170 with two).
-        const size_t smem = (size_t)NORM_RING * (a.residual ? 2 : 1) * (size_t)a.hidden * sizeof(T);
+        // eight a thread up to 2048 columns, two above (16 384 x 8192: 193 us with four and 256 threads, 170 with two and 512).
+        const size_t row = (a.residual ? 2 : 1) * (size_t)a.hidden * sizeof(T), room = (size_t)device_info().per_sm;
         const int vpt = eights <= 256 ? 1 : 2, threads = ((eights + vpt - 1) / vpt + 31) / 32 * 32;
-        const int per_sm = (int)std::min<size_t>((size_t)(1536 / threads), (size_t)device_info().per_sm / (smem + 2048));
+        // as many CTAs as are resident: 42 registers a thread, and 64 with two eights; 2 KB of an SM's room are not theirs
+        const int per_sm = (int)std::min<size_t>((size_t)((vpt == 1 ? 1536 : 1024) / threads), room / (NORM_RING * row + 2048));
         if (a.rows >= 16 * device_sms() && eights >= 256 && eights <= 2 * NORM_STREAM_NT && per_sm >= 2) {
-            if (vpt == 1) return launch_norm_stream<T, QUANT, 1>(a, threads, per_sm, smem, stream);
-            return launch_norm_stream<T, QUANT, 2>(a, threads, per_sm, smem, stream);
+            if (vpt == 1) return launch_norm_stream<T, QUANT, 1>(a, threads, per_sm, NORM_RING * row, stream);
+            return launch_norm_stream<T, QUANT, 2>(a, threads, per_sm, NORM_RING * row, stream);
         }
     }
     // A CTA a row.  Few rows: as few eights a thread as 512 threads allow, the shortest path through the kernel.  Many
