@@ -557,8 +557,9 @@ class BatchSampler:
 
     def step_hidden_async(self, head, uniforms, norm=None, stream=None, logit_scale=0.0, logit_softcap=0.0):
         """Queues norm (head.NormPlan, optional), head (head.HeadPlan) and one step on the logits it writes."""
-        if head.device != self.device or (norm is not None and norm.device != self.device):
-            raise ValueError("the plans are not on %s" % self.device)
+        for plan in (head, norm):
+            if plan is not None and self.device.index is not None and plan.device != self.device:
+                raise ValueError("the plans are not on %s" % self.device)
         u = np.ascontiguousarray(uniforms, dtype=np.float64)
         if u.shape != (self.rows,):
             raise ValueError("one uniform per row")

@@ -211,6 +211,52 @@ def test_adapters_beside_a_projection(rows, dtype):
             assert torch.equal(base, got)
 
 
+@pytest.mark.parametrize("dtype", [BF16, E4M3])
+@pytest.mark.parametrize("rows,vocab,hidden,n,rank", [
+    (3, 40, 65536, 2, 8),        # the widest row: rounds of either type
+    (128, 300, 64, 200, 32),     # nearly every row its own adapter: several segments of steps a tile, rows in place
+    (300, 700, 64, 400, 32),     # the same with sorted rows
+    (1000, 260, 64, 1, 16),      # one adapter over several tiles of rows
+    (40, 64, 64, 4096, 8),       # the largest table
+    (2100, 130, 128, 5, 24),     # more rows than one pass of the sort's threads
+])
+def test_head_at_the_ends_of_its_ranges(rows, vocab, hidden, n, rank, dtype):
+    s = head_inputs(rows, vocab, hidden, dtype, n, rank)
+    check_head(s)
+    s["ids"].copy_(torch.arange(rows, dtype=torch.int32) % (n + 1) - 1)
+    check_head(s)
+    s.pop("weight")
+    s.pop("weight_scales", None)
+    s["base"] = rand(9, rows, vocab)
+    check_head(s)
+
+
+def test_two_graphs_of_two_plans_and_more_rows_than_stay_in_place():
+    """The sorted form captured, ids changed between replays, beside another graph on another stream."""
+    made = []
+    for i in range(2):
+        s = head_inputs(200 + 90 * i, 900, 128, (BF16, E4M3)[i], 12, 16, seed=20 * i)
+        plan = head_plan(s)
+        plan.launch()
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            plan.launch()
+        made.append((s, plan, g, torch.cuda.Stream()))
+    for turn in range(3):
+        for i, (s, plan, g, st) in enumerate(made):
+            rows = s["ids"].shape[0]
+            s["ids"].copy_(torch.randint(-1, 12, (rows,), generator=torch.Generator().manual_seed(turn + 7 * i), dtype=torch.int32))
+        torch.cuda.synchronize()
+        for s, plan, g, st in made:
+            with torch.cuda.stream(st):
+                g.replay()
+        torch.cuda.synchronize()
+        for s, plan, g, st in made:
+            want, slack = R.head(**s)
+            R.check(plan.out, want, slack, turn)
+
+
 def test_ids_that_mean_no_adapter():
     s = head_inputs(70, 900, 128, BF16, 4, 16)
     plain = head_plan({k: s[k] for k in ("hidden", "weight")}).launch()
