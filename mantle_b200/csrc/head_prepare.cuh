@@ -233,6 +233,9 @@ __device__ __forceinline__ float shrink32(const HeadPrep& p, int adapter, int j0
     }
     const bf16_raw* arow = p.a + ((long long)adapter * p.rank + j0 + g) * p.hidden;
     const bool both = j0 + 8 < p.rank;  // (the rank may end after eight)
+    const int mine = rows[threadIdx.x >> 4];
+    float factor = p.gain ? p.gain[adapter] : 1.0f;
+    if (p.e4m3 && mine >= 0) factor *= p.x_scales[mine];
     float d[2][2][4] = {};
     const uint4 none = make_uint4(0, 0, 0, 0);
 #pragma unroll 4
@@ -261,15 +264,12 @@ __device__ __forceinline__ float shrink32(const HeadPrep& p, int adapter, int j0
         }
     }
     __syncthreads();
-    const int i = threadIdx.x >> 4, j = threadIdx.x & 15, r = rows[i];
+    const int i = threadIdx.x >> 4, j = threadIdx.x & 15;
+    if (mine < 0) return 0.0f;
     float v = 0.0f;
-    if (r >= 0) {
 #pragma unroll
-        for (int w = 0; w < SHRINK_WARPS; w++) v += sums[w][i][j];
-        if (p.gain) v *= p.gain[adapter];
-        if (p.e4m3) v *= p.x_scales[r];
-    }
-    return v;
+    for (int w = 0; w < SHRINK_WARPS; w++) v += sums[w][i][j];
+    return v * factor;
 }
 
 // u lies in memory as the tensor cores read it from shared memory without swizzle: blocks of 8 rows by 8 values (16
@@ -313,19 +313,19 @@ __global__ void __launch_bounds__(SHRINK_NT) head_shrink_kernel(const HeadPrep p
     store_u(p, j0 + (int)(threadIdx.x & 15), (int)blockIdx.x * WINDOW + (int)(threadIdx.x >> 4), v);
 }
 
-// Form for up to HERE_ROWS rows.  CTAs [0, units) x [0, chunks): a chunk of ranks of the rows of one adapter -- the
+// Form for up to HERE_ROWS rows.  CTAs [0, units) x [0, chunks) x [0, rows / 32): a chunk of ranks of up to 32 rows of one adapter -- the
 // blockIdx.x-th of those in use, in the order of their first rows -- and zeros for the others.  CTAs from `units` on:
 // the copy of x, where its rows do not start on 16 bytes.
 __global__ void __launch_bounds__(SHRINK_NT) head_shrink_here_kernel(const HeadPrep p) {
     __shared__ ShrinkSums sums;
     __shared__ __align__(16) int ids[HERE_ROWS];
     __shared__ int mine[HERE_ROWS], first_of[HERE_ROWS];
-    __shared__ int counts[2 * (HERE_ROWS / 32)];
+    __shared__ int counts[2 * (HERE_ROWS / 32)];  // of its first HERE_ROWS threads' warps, twice
     pdl_wait();
     pdl_trigger();  // not before: the projection reads W and x as soon as it starts
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if ((int)blockIdx.x >= p.units) {
-        if (blockIdx.y == 0)
+        if (blockIdx.y == 0 && blockIdx.z == 0)
             copy_rows(p, ((int)blockIdx.x - p.units) * SHRINK_WARPS + warp, p.copy_ctas * SHRINK_WARPS);
         return;
     }
@@ -354,7 +354,7 @@ __global__ void __launch_bounds__(SHRINK_NT) head_shrink_here_kernel(const HeadP
     __syncthreads();
     int in_use = 0;
     for (int w = 0; w < HERE_ROWS / 32; w++) in_use += counts[w];
-    if (blockIdx.x == 0 && blockIdx.y == 0) {
+    if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0) {
         if (tid < in_use) {
             HeadSlot s = {ids[first_of[tid]], 0, p.tile_cols, tid * p.tile_cols};
             p.slots[tid] = s;
@@ -372,16 +372,15 @@ __global__ void __launch_bounds__(SHRINK_NT) head_shrink_here_kernel(const HeadP
         for (int w = 0; w < warp; w++) at += counts[HERE_ROWS / 32 + w];
         if (use) mine[at] = tid;
     }
-    for (int i = tid; i < p.tile_cols * U_RANKS; i += SHRINK_NT)
+    for (int i = (int)blockIdx.z * SHRINK_NT + tid; i < p.tile_cols * U_RANKS; i += SHRINK_NT * (int)gridDim.z)
         if (ids[i / U_RANKS] != adapter) store_u(p, j0 + i % U_RANKS, u_row + i / U_RANKS, 0.0f);
     __syncthreads();
     int n = 0;
     for (int w = 0; w < HERE_ROWS / 32; w++) n += counts[HERE_ROWS / 32 + w];
-    for (int i = 0; i < n; i += 32) {
-        const float v = shrink32(p, adapter, j0, mine + i, sums);
-        if (i + (tid >> 4) < n) store_u(p, j0 + (tid & 15), u_row + mine[i + (tid >> 4)], v);
-        __syncthreads();
-    }
+    const int i = (int)blockIdx.z * 32;
+    if (i >= n) return;
+    const float v = shrink32(p, adapter, j0, mine + i, sums);
+    if (i + (tid >> 4) < n) store_u(p, j0 + (tid & 15), u_row + mine[i + (tid >> 4)], v);
 }
 
 // B of the adapters as the tensor cores read it, so that any run of 8 vocabulary rows of a chunk of 16 ranks is one

@@ -122,15 +122,25 @@ struct NormWeight {
             } else if constexpr (VEC) {
                 if (a.weight && !a.weight_f32 && c.has(j)) raw[j] = *reinterpret_cast<const uint4*>(static_cast<const bf16_raw*>(a.weight) + c.at(j, 0));
             } else {
-#pragma unroll
-                for (int e = 0; e < 8; e++) one[j][e] = one_of(a, c, j, e);
+                singles(a, c, j, one[j]);
             }
         }
     }
-    __device__ __forceinline__ float one_of(const NormArgs& a, const NormCols<VPT, VEC>& c, int j, int e) const {
-        if (!a.weight || !c.has(j, e)) return 1.0f;
-        return a.weight_f32 ? load1(static_cast<const float*>(a.weight) + c.at(j, e))
-                            : load1(static_cast<const bf16_raw*>(a.weight) + c.at(j, e));
+    // eight single columns: the type is asked for once, so that the loads go out together
+    template <typename P>
+    __device__ __forceinline__ void singles_of(const P* p, const NormCols<VPT, VEC>& c, int j, float w[8]) const {
+#pragma unroll
+        for (int e = 0; e < 8; e++) w[e] = c.has(j, e) ? load1(p + c.at(j, e)) : 1.0f;
+    }
+    __device__ __forceinline__ void singles(const NormArgs& a, const NormCols<VPT, VEC>& c, int j, float w[8]) const {
+        if (!a.weight) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) w[e] = 1.0f;
+        } else if (a.weight_f32) {
+            singles_of(static_cast<const float*>(a.weight), c, j, w);
+        } else {
+            singles_of(static_cast<const bf16_raw*>(a.weight), c, j, w);
+        }
     }
     __device__ __forceinline__ void get(const NormArgs& a, const NormCols<VPT, VEC>& c, int j, float w[8]) const {
         if constexpr (VEC) {
@@ -144,12 +154,11 @@ struct NormWeight {
             } else {
                 load8(static_cast<const bf16_raw*>(a.weight) + c.at(j, 0), w);
             }
-        } else {
+        } else if constexpr (EARLY) {
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                if constexpr (EARLY) w[e] = one[j][e];
-                else w[e] = one_of(a, c, j, e);
-            }
+            for (int e = 0; e < 8; e++) w[e] = one[j][e];
+        } else {
+            singles(a, c, j, w);
         }
 #pragma unroll
         for (int e = 0; e < 8; e++) w[e] += a.offset;
@@ -257,16 +266,17 @@ __device__ __forceinline__ void norm_finish(const NormArgs& a, long long row, co
                 }
             }
             __syncthreads();
-            for (int g = threadIdx.x; g < groups; g += blockDim.x)
-                scales[g] = max_nan(__fdiv_rn(__uint_as_float(group_max[g]), E4M3_MAX), E4M3_SCALE_MIN);
+            for (int g = threadIdx.x; g < groups; g += blockDim.x) {
+                const float scale = max_nan(__fdiv_rn(__uint_as_float(group_max[g]), E4M3_MAX), E4M3_SCALE_MIN);
+                scales[g] = scale;
+                group_max[g] = __float_as_uint(__frcp_rn(scale));
+            }
+            __syncthreads();
 #pragma unroll
             for (int j = 0; j < VPT; j++) {
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    if (!c.has(j, e)) continue;
-                    const float m = __uint_as_float(group_max[c.at(j, e) / MANTLE_NORM_GROUP]);
-                    s[j][e] *= __frcp_rn(max_nan(__fdiv_rn(m, E4M3_MAX), E4M3_SCALE_MIN));
-                }
+                for (int e = 0; e < 8; e++)
+                    if (c.has(j, e)) s[j][e] *= __uint_as_float(group_max[c.at(j, e) / MANTLE_NORM_GROUP]);
             }
         }
 #pragma unroll
@@ -297,7 +307,7 @@ __global__ void __launch_bounds__(WARP_ROW ? 128 : NORM_NT) norm_rows_kernel(con
     const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
     const T* res = a.residual ? static_cast<const T*>(a.residual) + row * a.residual_stride : nullptr;
     T* res_out = a.residual_out ? static_cast<T*>(a.residual_out) + row * a.residual_out_stride : nullptr;
-    constexpr bool EARLY = NormWeight<VPT, VEC>::EARLY;
+    constexpr bool EARLY = VPT <= 4;
     float s[VPT][8], r[EARLY ? VPT : 1][8];
     // all loads before the first use, as far as registers reach
 #pragma unroll
@@ -351,7 +361,7 @@ constexpr int NORM_RING = 2;          // (four deep measured the same)
 constexpr int NORM_STREAM_NT = 512;  // threads at most
 
 template <typename T, bool QUANT, int VPT>
-__global__ void __launch_bounds__(VPT == 1 ? NORM_STREAM_NT / 2 : NORM_STREAM_NT, VPT == 1 ? 6 : 2) norm_stream_kernel(const NormArgs a) {
+__global__ void __launch_bounds__(VPT == 1 ? NORM_STREAM_NT / 2 : NORM_STREAM_NT, VPT == 1 ? 6 : VPT == 2 ? 2 : 1) norm_stream_kernel(const NormArgs a) {
     extern __shared__ __align__(128) char ring[];  // [NORM_RING][x, residual][row_bytes]
     __shared__ float part[2][2][32];               // a row's, and the next one's
     __shared__ uint64_t full[NORM_RING];
@@ -454,15 +464,17 @@ int launch_norm_as(const NormArgs& a, cudaStream_t stream) {
         if (many && eights <= 128) return launch_norm_kernel(norm_rows_kernel<T, QUANT, 4, VEC, true>, a, grid, 128, 0, stream);
     }
     if constexpr (VEC) {
-        // The ring: where an SM gets several rows, and a row is worth a bulk copy.  Two CTAs of it have to fit.  One
-        // eight a thread up to 2048 columns, two above (16 384 x 8192: 193 us with four and 256 threads, 170 with two and 512).
+        // The ring: where a CTA gets several rows, and a row is worth a bulk copy.  One eight a thread up to 2048
+        // columns, two up to 8192 (16 384 x 8192: 193 us with four and 256 threads, 170 with two and 512), four above.
         const size_t row = (a.residual ? 2 : 1) * (size_t)a.hidden * sizeof(T), room = (size_t)device_info().per_sm;
-        const int vpt = eights <= 256 ? 1 : 2, threads = ((eights + vpt - 1) / vpt + 31) / 32 * 32;
-        // as many CTAs as are resident: 42 registers a thread, and 64 with two eights; 2 KB of an SM's room are not theirs
-        const int per_sm = (int)std::min<size_t>((size_t)((vpt == 1 ? 1536 : 1024) / threads), room / (NORM_RING * row + 2048));
-        if (a.rows >= 16 * device_sms() && eights >= 256 && eights <= 2 * NORM_STREAM_NT && per_sm >= 2) {
+        const int vpt = eights <= 256 ? 1 : eights <= 2 * NORM_STREAM_NT ? 2 : 4, threads = ((eights + vpt - 1) / vpt + 31) / 32 * 32;
+        // as many CTAs as are resident: 42 registers a thread, 64 with two eights, 128 with four; 2 KB of an SM's room are
+        // not theirs
+        const int per_sm = (int)std::min<size_t>((size_t)((vpt == 1 ? 1536 : vpt == 2 ? 1024 : 512) / threads), room / (NORM_RING * row + 2048));
+        if (eights >= 256 && eights <= 4 * NORM_STREAM_NT && per_sm >= 1 && a.rows >= 3ll * device_sms() * per_sm) {
             if (vpt == 1) return launch_norm_stream<T, QUANT, 1>(a, threads, per_sm, NORM_RING * row, stream);
-            return launch_norm_stream<T, QUANT, 2>(a, threads, per_sm, NORM_RING * row, stream);
+            if (vpt == 2) return launch_norm_stream<T, QUANT, 2>(a, threads, per_sm, NORM_RING * row, stream);
+            return launch_norm_stream<T, QUANT, 4>(a, threads, per_sm, NORM_RING * row, stream);
         }
     }
     // A CTA a row.  Few rows: as few eights a thread as 512 threads allow, the shortest path through the kernel.  Many
