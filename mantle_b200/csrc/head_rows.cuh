@@ -14,8 +14,8 @@
 // accumulators out of tensor memory, add them up in registers and write the finished tile while the next one is
 // computed.  Warp 10 works out, a lane each, what every step of the tile's adapters copies and multiplies, ahead of the
 // three that issue: an instruction that starts a copy or a product costs its warp some hundred cycles, and what
-// stands around it comes on top (one adapter's step of 64 rows: 490 cycles to copy and 380 to multiply; it has
-// 4 KB of B, which HBM delivers in 170).
+// stands around it comes on top (one adapter's step of 64 rows took a single copying warp 490 cycles; it has 4 KB of
+// B, which HBM delivers in 170).
 //
 // Pairs.  W comes from HBM once, but x from L2 for every 128 vocabulary rows: at 256 rows that is twice W's bytes,
 // and what L2 can hand out (about 10 TB/s) bounds the kernel long before HBM or the tensor cores do.  From 65 rows
@@ -63,7 +63,7 @@ struct __align__(16) HeadCtl {
 struct HeadArgs {
     int rows, vocab, w_steps, tile_cols, row_tiles, v_tiles;
     int front_is_ours;                // prepare kernels of the same call stand in front
-    int slots_on, sorted, copied;  // adapters; perm and x come from the kernel in front
+    int slots_on, sorted, copied;     // adapters; perm comes from the kernels in front; x does
     int chunks, u_rows, u_box;        // u_box: rows of u of one copy
     int pack, pack_bytes;             // adapters' steps in one stage, and the room of each
     int b_rows;                       // 128-byte rows of one chunk of an adapter's B
@@ -85,7 +85,7 @@ struct HeadMaps {
 
 // ---- the instructions
 //
-// Warps 8 and 9 run as whole warps, all lanes with the same values, and only the instructions that act take a predicate
+// Warps 8, 9 and 11 run as whole warps, all lanes with the same values, and only the instructions that act take a predicate
 // (`on`, true in one lane): the operands then live in the uniform registers that these instructions want.  As the
 // code of a single thread every stage's four products took 515 cycles to issue, whatever their size: that alone was
 // as long as W takes to come from HBM.
@@ -96,7 +96,7 @@ __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
 __device__ __forceinline__ void mbar_arrive_on(uint32_t bar, bool on) {
     asm volatile("{.reg .pred q; setp.ne.b32 q, %1, 0; @q mbarrier.arrive.shared::cta.b64 _, [%0];}" ::"r"(bar), "r"((int)on) : "memory");
 }
-// Announces the bytes of a stage's copies; with `arrive` the announcement is complete.
+// Announces the bytes of a stage's copies, and that these are all; the next one: that there are more to come.
 __device__ __forceinline__ void mbar_expect_on(uint32_t bar, uint32_t bytes, bool on) {
     asm volatile("{.reg .pred q; setp.ne.b32 q, %2, 0; @q mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;}" ::"r"(bar), "r"(bytes), "r"((int)on) : "memory");
 }
