@@ -572,9 +572,7 @@ class BatchSampler:
     def step_hidden(self, head, rngs, **kw):
         """step() from the hidden state that `head` (behind `norm`) reads."""
         self.step_hidden_async(head, self.draw(rngs), **kw)
-        torch.cuda.current_stream(self.device).synchronize()
-        n, e, status = self.results()
-        return n, e
+        return self._finish(kw.get("stream"))
 
     def results(self):
         """(next tokens, ended flags, status word) of the last step, as numpy arrays (copies)."""
@@ -589,6 +587,10 @@ class BatchSampler:
     def step(self, logits, rngs, **kw):
         """draw + step_async + synchronise + results: one iteration of the reference's loop for the batch."""
         self.step_async(logits, self.draw(rngs), **kw)
-        torch.cuda.current_stream(self.device).synchronize()
+        return self._finish(kw.get("stream"))
+
+    def _finish(self, stream):
+        # the stream that the step was queued on: until it is done the pinned results are those of the step before
+        (torch.cuda.current_stream(self.device) if stream is None else stream).synchronize()
         n, e, status = self.results()
         return n, e

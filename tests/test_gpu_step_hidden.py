@@ -1,0 +1,51 @@
+"""BatchSampler.step and step_hidden where the other tests do not reach: other streams, refusals, statuses."""
+import numpy as np
+import pytest
+import torch
+
+from mantle_b200 import head as H
+from mantle_b200 import native, sampler
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+BF16, F32, E4M3 = torch.bfloat16, torch.float32, torch.float8_e4m3fn
+SLEEP = 200_000_000  # cycles, about a tenth of a second
+
+
+def rand(seed, *shape):
+    g = torch.Generator(device="cpu")
+    g.manual_seed(seed)
+    return torch.randn(shape, generator=g, dtype=F32).to(DEV)
+
+
+def started(rows, vocab, **kw):
+    b = sampler.BatchSampler(rows, vocab, 256, [7], **{"device": DEV, **kw})
+    for i in range(rows):
+        b.set_row(i, sampler.SamplerConfig(seed=i, temperature=0.9, top_k=20, top_p=0.95), [i, i + 1])
+    return b
+
+
+def generators(rows):
+    return [np.random.default_rng(i).random for i in range(rows)]
+
+
+@pytest.mark.parametrize("hidden_state", [False, True])
+def test_steps_on_a_busy_side_stream(hidden_state):
+    """The tokens are this step's, not the ones that the step before left in pinned memory."""
+    rows, vocab, hidden = 8, 2000, 64
+    x, w = rand(1, rows, hidden).to(BF16), rand(2, vocab, hidden).to(BF16)
+    plan = H.HeadPlan(x, w)
+    logits = plan.launch()
+    side = torch.cuda.Stream()
+    got_by, ref_by = started(rows, vocab), started(rows, vocab)
+    got_rng, ref_rng = generators(rows), generators(rows)
+    torch.cuda.synchronize()
+    for _ in range(3):
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(SLEEP)
+        got, ended = (got_by.step_hidden(plan, got_rng, stream=side) if hidden_state
+                      else got_by.step(logits, got_rng, stream=side))
+        ref, ref_ended = ref_by.step(logits, ref_rng)
+        assert np.array_equal(got, ref) and np.array_equal(ended, ref_ended)
+    got_by.close()
+    ref_by.close()
