@@ -47,6 +47,40 @@ size_t workspace_bound(int rows) {
     return split_rows * (4096 * 8 + 64 * 4) + 4096;
 }
 
+// What a step samples from, and the workspace it needs; refuses, before anything is queued, what the sampling kernels
+// would refuse.
+int step_batch(const MantleBatchSampler* s, const void* dev_logits, int dtype, int64_t row_stride, float logit_scale,
+               float logit_softcap, MantleSampleBatch* b, size_t* need) {
+    int max_k = 1;
+    for (int r = 0; r < s->rows; r++) {
+        const MantleSampleParams& p = s->h_params[0][r];  // (both buffers hold the same configurations)
+        if (!s->ended[r]) {
+            const int k = p.top_k < s->vocab ? p.top_k : s->vocab;  // sampler.go:147
+            if (!mantle_internal_argmax_shortcut(p) && k > max_k) max_k = k;
+        }
+    }
+    memset(b, 0, sizeof *b);
+    b->logits = dev_logits;
+    b->dtype = dtype;
+    b->rows = s->rows;
+    b->vocab = s->vocab;
+    b->max_top_k = max_k;
+    b->row_stride = row_stride;
+    b->history = s->d_history;
+    b->hist_len = s->d_hist_len;
+    b->hist_stride = s->cap;
+    b->exclude = s->n_stop > 0 ? s->d_stop : nullptr;  // excludePenalty = StopTokens (engine.go:233)
+    b->n_exclude = s->n_stop;
+    b->params = s->d_params;
+    b->next = s->d_next;
+    b->status = s->d_status;
+    b->skip = s->d_ended;
+    b->logit_scale = logit_scale;
+    b->logit_softcap = logit_softcap;
+    const int rc = mantleCudaSamplerWorkspaceBytes(b, need);
+    return rc ? rc : *need > s->d_ws_bytes ? kInvalid : 0;
+}
+
 }  // namespace
 
 extern "C" MantleBatchSampler* mantleBatchSamplerNew(int rows, int vocab, int hist_capacity, const int64_t* stop,
@@ -195,6 +229,10 @@ extern "C" int mantleBatchSamplerStep(MantleBatchSampler* s, const void* dev_log
                                       const double* uniforms, float logit_scale, float logit_softcap,
                                       mantleCudaStream_t stream_) {
     if (!s || !dev_logits || !uniforms || row_stride < s->vocab) return kInvalid;
+    MantleSampleBatch b;
+    size_t need = 0;
+    int rc = step_batch(s, dev_logits, dtype, row_stride, logit_scale, logit_softcap, &b, &need);
+    if (rc) return rc;
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
     // this step's parameter records: the rows' configurations and their uniform draws
     const int t = s->turn;
@@ -202,41 +240,11 @@ extern "C" int mantleBatchSamplerStep(MantleBatchSampler* s, const void* dev_log
     cudaError_t e = cudaEventSynchronize(s->params_free[t]);  // the upload of two steps ago; normally long done
     if (e != cudaSuccess) return (int)e;
     MantleSampleParams* hp = s->h_params[t];
-    int max_k = 1;
-    for (int r = 0; r < s->rows; r++) {
-        hp[r].uniform = uniforms[r];
-        if (!s->ended[r]) {
-            const int k = hp[r].top_k < s->vocab ? hp[r].top_k : s->vocab;  // sampler.go:147
-            if (!mantle_internal_argmax_shortcut(hp[r]) && k > max_k) max_k = k;
-        }
-    }
+    for (int r = 0; r < s->rows; r++) hp[r].uniform = uniforms[r];
     e = cudaMemcpyAsync(s->d_params, hp, (size_t)s->rows * sizeof(MantleSampleParams), cudaMemcpyHostToDevice, stream);
     if (e == cudaSuccess) e = cudaEventRecord(s->params_free[t], stream);
     if (e != cudaSuccess) return (int)e;
 
-    MantleSampleBatch b;
-    memset(&b, 0, sizeof b);
-    b.logits = dev_logits;
-    b.dtype = dtype;
-    b.rows = s->rows;
-    b.vocab = s->vocab;
-    b.max_top_k = max_k;
-    b.row_stride = row_stride;
-    b.history = s->d_history;
-    b.hist_len = s->d_hist_len;
-    b.hist_stride = s->cap;
-    b.exclude = s->n_stop > 0 ? s->d_stop : nullptr;  // excludePenalty = StopTokens (engine.go:233)
-    b.n_exclude = s->n_stop;
-    b.params = s->d_params;
-    b.next = s->d_next;
-    b.status = s->d_status;
-    b.skip = s->d_ended;
-    b.logit_scale = logit_scale;
-    b.logit_softcap = logit_softcap;
-    size_t need = 0;
-    int rc = mantleCudaSamplerWorkspaceBytes(&b, &need);
-    if (rc) return rc;
-    if (need > s->d_ws_bytes) return kInvalid;
     rc = mantleCudaSampleRows(&b, need ? s->d_ws : nullptr, need, stream_);
     if (rc) return rc;
     // toks = append(toks, next), or the end of the row on a stop token (engine.go:244-250)
@@ -266,6 +274,9 @@ extern "C" int mantleBatchSamplerStepHidden(MantleBatchSampler* s, const MantleN
         fault = "the head does not read what the norm writes";
     if (!fault && norm && norm->out_scale && (norm->out_scale != head->hidden_scales || norm->scale_group != 0 || norm->scale_stride != 1))
         fault = "the head wants the norm's scales, one a row and one behind the other";
+    MantleSampleBatch b;
+    if (!fault && step_batch(s, head->out, head->out_dtype, head->out_stride, logit_scale, logit_softcap, &b, &need))
+        fault = "logit_scale must be finite and not negative, logit_softcap finite";
     if (fault) {
         mantle_internal_set_last_error(fault);
         return kInvalid;

@@ -49,3 +49,30 @@ def test_steps_on_a_busy_side_stream(hidden_state):
         assert np.array_equal(got, ref) and np.array_equal(ended, ref_ended)
     got_by.close()
     ref_by.close()
+
+
+@pytest.mark.parametrize("post", [dict(logit_scale=-1.0), dict(logit_scale=float("nan")), dict(logit_scale=float("inf")),
+                                  dict(logit_softcap=float("inf")), dict(logit_softcap=float("-inf"))])
+def test_a_refused_step_has_launched_nothing(post):
+    """The norm in front would add x to the residual once more on the retry."""
+    rows, vocab, hidden = 8, 2000, 64
+    x, r, w = rand(1, rows, hidden).to(BF16), rand(2, rows, hidden).to(BF16), rand(3, vocab, hidden).to(BF16)
+    norm = H.NormPlan(x, residual=r, residual_out=r)
+    plan = H.HeadPlan(norm.out, w)
+    norm.out.fill_(3.0)
+    plan.out.fill_(5.0)
+    r0 = r.clone()
+    by, ref_by = started(rows, vocab), started(rows, vocab)
+    rng, ref_rng = generators(rows), generators(rows)
+    with pytest.raises(native.CudaError):
+        by.step_hidden_async(plan, np.zeros(rows), norm=norm, **post)
+    with pytest.raises(native.CudaError):
+        by.step_async(plan.out, np.zeros(rows), **post)
+    torch.cuda.synchronize()
+    assert torch.equal(r, r0) and bool((norm.out == 3.0).all()) and bool((plan.out == 5.0).all())
+    got, _ = by.step_hidden(plan, rng, norm=norm)
+    assert torch.equal(r, (x.float() + r0.float()).to(BF16))
+    ref, _ = ref_by.step(plan.out, ref_rng)
+    assert np.array_equal(got, ref)
+    by.close()
+    ref_by.close()
