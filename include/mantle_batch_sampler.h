@@ -86,7 +86,9 @@ int mantleBatchSamplerStep(MantleBatchSampler* s, const void* dev_logits, int dt
  * adapters of the rows' requests, and the step on the logits it writes, one behind the other on `stream`.
  * head->rows and head->vocab are the sampler's, norm->out is what the head reads (hidden_rows), with the same
  * rows, width, type, stride and scales; workspace as for mantleCudaHeadRows.  cudaErrorInvalidValue, with
- * nothing launched, where any of it does not fit.
+ * nothing launched, where any of it does not fit.  The bits of norm->status and head->status, which may be NULL, are
+ * OR-ed into the status that Results reports: with MANTLE_SAMPLE_STATUS_TIMEOUT among them the step's tokens, and the
+ * histories that they were appended to, are not valid.
  */
 int mantleBatchSamplerStepHidden(MantleBatchSampler* s, const MantleNormBatch* norm, const MantleHeadBatch* head,
                                  void* workspace, size_t workspace_bytes, const double* uniforms, float logit_scale,
@@ -96,7 +98,7 @@ int mantleBatchSamplerStepHidden(MantleBatchSampler* s, const MantleNormBatch* n
  * The last step's results, valid once `stream` has been synchronised and until the next Step:
  * next[r] is the token row r sampled (-1 for a row that had already ended), ended[r] is 1 once
  * the row has sampled a stop token or was ended; status is the OR of the kernels' status bits
- * since the sampler was made.  The pointers are pinned host memory owned by the sampler.
+ * since the sampler was made, with those of StepHidden's norm and head.  The pointers are pinned host memory owned by the sampler.
  * dev_next is the same token array on the device, for a model that feeds from it directly.
  */
 int mantleBatchSamplerResults(MantleBatchSampler* s, const int32_t** next, const int32_t** ended, int32_t* status,

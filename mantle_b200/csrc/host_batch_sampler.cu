@@ -225,14 +225,9 @@ extern "C" int mantleBatchSamplerCanUseDeviceGreedy(const MantleBatchSampler* s,
     return p.greedy && p.repeat_penalty <= 1.0f;
 }
 
-extern "C" int mantleBatchSamplerStep(MantleBatchSampler* s, const void* dev_logits, int dtype, int64_t row_stride,
-                                      const double* uniforms, float logit_scale, float logit_softcap,
-                                      mantleCudaStream_t stream_) {
-    if (!s || !dev_logits || !uniforms || row_stride < s->vocab) return kInvalid;
-    MantleSampleBatch b;
-    size_t need = 0;
-    int rc = step_batch(s, dev_logits, dtype, row_stride, logit_scale, logit_softcap, &b, &need);
-    if (rc) return rc;
+// Queues a step on a checked batch; more_status: words of the kernels in front, whose bits become the step's.
+static int queue_step(MantleBatchSampler* s, const MantleSampleBatch& b, size_t need, const double* uniforms,
+                      const int32_t* const more_status[2], mantleCudaStream_t stream_) {
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
     // this step's parameter records: the rows' configurations and their uniform draws
     const int t = s->turn;
@@ -245,16 +240,27 @@ extern "C" int mantleBatchSamplerStep(MantleBatchSampler* s, const void* dev_log
     if (e == cudaSuccess) e = cudaEventRecord(s->params_free[t], stream);
     if (e != cudaSuccess) return (int)e;
 
-    rc = mantleCudaSampleRows(&b, need ? s->d_ws : nullptr, need, stream_);
+    int rc = mantleCudaSampleRows(&b, need ? s->d_ws : nullptr, need, stream_);
     if (rc) return rc;
     // toks = append(toks, next), or the end of the row on a stop token (engine.go:244-250)
-    rc = mantleCudaHistoryAppendRows(s->d_history, s->d_hist_len, s->cap, s->rows, s->d_next, s->keep,
-                                     s->n_stop > 0 ? s->d_stop : nullptr, s->n_stop, s->d_ended, stream_);
+    rc = mantle_internal_history_append(s->d_history, s->d_hist_len, s->cap, s->rows, s->d_next, s->keep,
+                                        s->n_stop > 0 ? s->d_stop : nullptr, s->n_stop, s->d_ended, s->d_status, more_status,
+                                        stream_);
     if (rc) return rc;
     e = cudaMemcpyAsync(s->h_next, s->d_next, (size_t)s->rows * 4, cudaMemcpyDeviceToHost, stream);
     if (e == cudaSuccess) e = cudaMemcpyAsync(s->h_ended, s->d_ended, (size_t)s->rows * 4, cudaMemcpyDeviceToHost, stream);
     if (e == cudaSuccess) e = cudaMemcpyAsync(s->h_status, s->d_status, 4, cudaMemcpyDeviceToHost, stream);
     return (int)e;
+}
+
+extern "C" int mantleBatchSamplerStep(MantleBatchSampler* s, const void* dev_logits, int dtype, int64_t row_stride,
+                                      const double* uniforms, float logit_scale, float logit_softcap,
+                                      mantleCudaStream_t stream) {
+    if (!s || !dev_logits || !uniforms || row_stride < s->vocab) return kInvalid;
+    MantleSampleBatch b;
+    size_t need = 0;
+    const int rc = step_batch(s, dev_logits, dtype, row_stride, logit_scale, logit_softcap, &b, &need);
+    return rc ? rc : queue_step(s, b, need, uniforms, nullptr, stream);
 }
 
 extern "C" int mantleBatchSamplerStepHidden(MantleBatchSampler* s, const MantleNormBatch* norm, const MantleHeadBatch* head,
@@ -281,11 +287,19 @@ extern "C" int mantleBatchSamplerStepHidden(MantleBatchSampler* s, const MantleN
         mantle_internal_set_last_error(fault);
         return kInvalid;
     }
-    rc = norm ? mantleCudaNormRows(norm, stream) : 0;
+    // a wait that runs out in front of the sampler is the step's: without a word of its own a batch takes the sampler's
+    MantleHeadBatch h = *head;
+    if (!h.status) h.status = s->d_status;
+    if (norm) {
+        MantleNormBatch n = *norm;
+        if (!n.status) n.status = s->d_status;
+        rc = mantleCudaNormRows(&n, stream);
+        if (rc) return rc;
+    }
+    rc = mantleCudaHeadRows(&h, workspace, workspace_bytes, stream);
     if (rc) return rc;
-    rc = mantleCudaHeadRows(head, workspace, workspace_bytes, stream);
-    if (rc) return rc;
-    return mantleBatchSamplerStep(s, head->out, head->out_dtype, head->out_stride, uniforms, logit_scale, logit_softcap, stream);
+    const int32_t* const more_status[2] = {norm ? norm->status : nullptr, head->status};
+    return queue_step(s, b, need, uniforms, more_status, stream);
 }
 
 extern "C" int mantleBatchSamplerResults(MantleBatchSampler* s, const int32_t** next, const int32_t** ended,

@@ -12,6 +12,11 @@ __attribute__((visibility("hidden"))) void mantle_internal_set_last_error(const 
 // What is wrong with a norm's batch; nullptr: nothing.
 __attribute__((visibility("hidden"))) const char* mantle_internal_norm_fault(const MantleNormBatch* b);
 
+// mantleCudaHistoryAppendRows, which also ORs more_status' words (either may be null) into *status.
+__attribute__((visibility("hidden"))) int mantle_internal_history_append(
+    int32_t* history, int32_t* hist_len, int hist_stride, int rows, const int32_t* next, int keep, const int32_t* stop, int n_stop,
+    int32_t* done, int32_t* status, const int32_t* const more_status[2], mantleCudaStream_t stream);
+
 // NewSampler's normalisation, internal/logits/sampler.go:61-83.
 static inline void mantle_internal_normalise(const MantleSamplerConfig& cfg, MantleSampleParams* p) {
     memset(p, 0, sizeof *p);

@@ -370,16 +370,25 @@ extern "C" int mantleCudaLogitPostprocessRowsF32(float* logits, int rows, int vo
     return (int)cudaGetLastError();
 }
 
-extern "C" int mantleCudaHistoryAppendRows(int32_t* history, int32_t* hist_len, int hist_stride, int rows,
-                                          const int32_t* next, int keep, const int32_t* stop, int n_stop,
-                                          int32_t* done, mantleCudaStream_t stream_) {
+int mantle_internal_history_append(int32_t* history, int32_t* hist_len, int hist_stride, int rows, const int32_t* next, int keep,
+                                   const int32_t* stop, int n_stop, int32_t* done, int32_t* status,
+                                   const int32_t* const more_status[2], mantleCudaStream_t stream_) {
     if (!history || !hist_len || !next || rows <= 0 || hist_stride < 2) return kInvalid;
     if (keep < 0 || keep > hist_stride / 2 || n_stop < 0 || (n_stop > 0 && !stop)) return kInvalid;
     const long long threads = (long long)rows * 32;
     if ((threads + 255) / 256 > 0x7fffffffLL) return kInvalid;
+    MoreStatus more = {status, {nullptr, nullptr}};
+    if (status && more_status) more.from[0] = more_status[0], more.from[1] = more_status[1];
     history_append_rows_kernel<<<(int)((threads + 255) / 256), 256, 0, static_cast<cudaStream_t>(stream_)>>>(
-        history, hist_len, hist_stride, rows, next, keep, stop, n_stop, done);
+        history, hist_len, hist_stride, rows, next, keep, stop, n_stop, done, more);
     return (int)cudaGetLastError();
+}
+
+extern "C" int mantleCudaHistoryAppendRows(int32_t* history, int32_t* hist_len, int hist_stride, int rows,
+                                          const int32_t* next, int keep, const int32_t* stop, int n_stop,
+                                          int32_t* done, mantleCudaStream_t stream_) {
+    return mantle_internal_history_append(history, hist_len, hist_stride, rows, next, keep, stop, n_stop, done, nullptr,
+                                          nullptr, stream_);
 }
 
 extern "C" int mantleCudaArgMaxRowsF32(const float* x, int rows, int n, int64_t row_stride, int* out_idx,

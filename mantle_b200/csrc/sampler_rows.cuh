@@ -187,10 +187,20 @@ __global__ void __launch_bounds__(PENALTY_NT) penalty_rows_kernel(const KArgs a)
 // leaves the loop before it appends; rows already done stay untouched.  A full buffer first
 // moves its `keep` most recent ids to the front (keep <= hist_stride / 2, so the two ranges
 // never overlap): the penalty window, the last repeat_last_n ids, is unchanged while keep
-// covers it.
+// covers it.  `more`: status words of the kernels in front of the sampler (the norm's, the head's; either may be null),
+// which the step's own word takes over.
+struct MoreStatus {
+    int32_t* status;
+    const int32_t* from[2];
+};
 __global__ void __launch_bounds__(256) history_append_rows_kernel(int32_t* history, int32_t* hist_len, int hist_stride,
                                                                   int rows, const int32_t* next, int keep,
-                                                                  const int32_t* stop, int n_stop, int32_t* done) {
+                                                                  const int32_t* stop, int n_stop, int32_t* done,
+                                                                  MoreStatus more) {
+    if (blockIdx.x == 0 && threadIdx.x < 2 && more.from[threadIdx.x]) {
+        const int32_t bits = *more.from[threadIdx.x];
+        if (bits) atomicOr(more.status, bits);
+    }
     const int row = (int)((blockIdx.x * (unsigned)blockDim.x + threadIdx.x) >> 5);
     const int lane = threadIdx.x & 31;
     if (row >= rows) return;

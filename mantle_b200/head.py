@@ -86,8 +86,26 @@ class _Plan:
             _check(self.lib, rc, self._name)
 
 
+    def check(self):
+        """Raises where a wait inside one of the launches so far ran out, whose outputs are then not valid, and clears
+        that mark.  Waits for the device's current stream: launches on others have to be done before."""
+        with torch.cuda.device(self._index):
+            bits = int(self.status.item())
+            if bits:
+                self.status.zero_()
+                raise RuntimeError("%s: a wait inside the kernel ran out (status %d)" % (self._name, bits))
+
+    def _status(self, status):
+        if status is None:
+            status = torch.zeros(1, dtype=torch.int32, device=self.device)
+        else:
+            _vector(status, "status", 1, (torch.int32,), self.device)
+        self.status = status
+        return status.data_ptr()
+
+
 class NormOutputs:
-    __slots__ = ("out", "scales", "residual_out")
+    __slots__ = ("out", "scales", "residual_out", "status")
 
 
 class NormPlan(_Plan):
@@ -99,10 +117,12 @@ class NormPlan(_Plan):
                  residual themselves may be given)
     out_dtype    None: x's type (out may be x itself).  torch.float8_e4m3fn: 8 bits, `scales` [rows, 1] float32 for
                  scale_group 0, [rows, ceil(hidden / 128)] for scale_group 128; value = out * scale
+    status       optional [1] int32 on the device, made here unless given: not 0 once a wait inside a launch has run out
+                 (check() says so; several plans may share one)
     """
 
     def __init__(self, x, weight=None, residual=None, eps=1e-6, weight_offset=0.0, out_dtype=None, scale_group=0,
-                 out=None, scales=None, residual_out=None):
+                 out=None, scales=None, residual_out=None, status=None):
         dtype, x_stride = _rows(x, "x", (torch.float32, torch.bfloat16))
         dev = x.device
         self._bind(dev)
@@ -148,8 +168,7 @@ class NormPlan(_Plan):
                 in_place = (n, m) in (("out", "x"), ("residual_out", "x"), ("residual_out", "residual")) and _same(t, u)
                 if _overlap(t, u) and not in_place:
                     raise ValueError("%s overlaps %s" % (n, m))
-        self.status = torch.zeros(1, dtype=torch.int32, device=dev)
-        b.status = self.status.data_ptr()
+        b.status = self._status(status)
         self.rows, self.hidden = rows, hidden
         self.out, self.scales, self.residual_out = out, scales, residual_out
         self.keep = [x, weight, residual]
@@ -157,7 +176,7 @@ class NormPlan(_Plan):
         self._args = (C.byref(b),)
         self._fn, self._name = self.lib.mantleCudaNormRows, "mantleCudaNormRows"
         o = NormOutputs()
-        o.out, o.scales, o.residual_out = out, scales, residual_out
+        o.out, o.scales, o.residual_out, o.status = out, scales, residual_out, self.status
         self._outputs = o
 
     def launch(self, stream=None):
@@ -167,7 +186,7 @@ class NormPlan(_Plan):
 
 
 def norm_rows(x, weight=None, stream=None, **kw):
-    """One-shot form of NormPlan."""
+    """One-shot form of NormPlan.  Its outputs carry `status`, which is not 0 where a wait inside the kernel ran out."""
     with torch.cuda.device(x.device), torch.cuda.stream(stream):  # outputs belong to the stream that writes them
         return NormPlan(x, weight, **kw).launch()
 
@@ -231,10 +250,11 @@ class HeadPlan(_Plan):
     base           instead of weight: [rows, vocab] of out_dtype, to which the adapters' part is added (out may be base)
     adapters, adapter_ids   a table and the [rows] int32 ids of the requests' adapters; an id outside the table: none
     out_dtype      float32 or bfloat16
+    status         as in NormPlan
     """
 
     def __init__(self, hidden, weight=None, hidden_scales=None, weight_scales=None, adapters=None, adapter_ids=None,
-                 base=None, out_dtype=None, out=None):
+                 base=None, out_dtype=None, out=None, status=None):
         dtype, b_stride = _rows(hidden, "hidden", (torch.bfloat16, torch.float8_e4m3fn))
         dev = hidden.device
         self._bind(dev)
@@ -292,8 +312,7 @@ class HeadPlan(_Plan):
         for t in reads:
             if t is not None and _overlap(out, t) and not (t is base and _same(out, base)):
                 raise ValueError("out overlaps an input")
-        self.status = torch.zeros(1, dtype=torch.int32, device=dev)
-        b.status = self.status.data_ptr()
+        b.status = self._status(status)
         n = C.c_size_t(0)
         with torch.cuda.device(dev):
             _check(self.lib, self.lib.mantleCudaHeadWorkspaceBytes(C.byref(b), C.byref(n)), "mantleCudaHeadWorkspaceBytes")
@@ -316,7 +335,7 @@ class HeadPlan(_Plan):
 
 
 def head_logits(hidden, weight=None, stream=None, **kw):
-    """One-shot form of HeadPlan."""
+    """One-shot form of HeadPlan.  Pass `status` to learn of a wait inside the kernel that ran out."""
     with torch.cuda.device(hidden.device), torch.cuda.stream(stream):
         plan = HeadPlan(hidden, weight, **kw)
         return plan.launch()

@@ -570,7 +570,9 @@ class BatchSampler:
         native.check(rc, "mantleBatchSamplerStepHidden")
 
     def step_hidden(self, head, rngs, **kw):
-        """step() from the hidden state that `head` (behind `norm`) reads."""
+        """step() from the hidden state that `head` (behind `norm`) reads.  RuntimeError where a wait in either has run out
+        (also in a launch before, until the plan's check() has said so): the sampler's rows have to be started anew in
+        another BatchSampler."""
         self.step_hidden_async(head, self.draw(rngs), **kw)
         return self._finish(kw.get("stream"))
 
@@ -593,4 +595,6 @@ class BatchSampler:
         # the stream that the step was queued on: until it is done the pinned results are those of the step before
         (torch.cuda.current_stream(self.device) if stream is None else stream).synchronize()
         n, e, status = self.results()
+        if status & native.STATUS_TIMEOUT:
+            raise RuntimeError("a wait in the norm or the head ran out: this step's tokens and histories are not valid")
         return n, e

@@ -76,3 +76,41 @@ def test_a_refused_step_has_launched_nothing(post):
     assert np.array_equal(got, ref)
     by.close()
     ref_by.close()
+
+
+@pytest.mark.parametrize("which", ["norm", "head"])
+def test_a_wait_that_ran_out_is_the_steps_error(which):
+    """The mark that such a wait leaves in a plan's status word, put there by hand."""
+    rows, vocab, hidden = 8, 2000, 64
+    x, w = rand(1, rows, hidden).to(BF16), rand(2, vocab, hidden).to(BF16)
+    norm = H.NormPlan(x)
+    plan = H.HeadPlan(norm.out, w)
+    by = started(rows, vocab)
+    rng = generators(rows)
+    by.step_hidden(plan, rng, norm=norm)
+    assert by.results()[2] == 0
+    bad = {"norm": norm, "head": plan}[which]
+    bad.status.fill_(native.STATUS_TIMEOUT)
+    with pytest.raises(RuntimeError, match="ran out"):
+        by.step_hidden(plan, rng, norm=norm)
+    assert by.results()[2] & native.STATUS_TIMEOUT
+    with pytest.raises(RuntimeError, match="ran out"):
+        bad.check()
+    norm.check()  # said once
+    plan.check()
+    by.close()
+    by = started(rows, vocab)
+    by.step_hidden(plan, rng, norm=norm)
+    by.close()
+
+
+def test_status_words_of_the_one_shot_forms():
+    x, w = rand(1, 8, 64).to(BF16), rand(2, 100, 64).to(BF16)
+    word = torch.zeros(1, dtype=torch.int32, device=DEV)
+    o = H.norm_rows(x, status=word)
+    assert o.status is word and int(H.norm_rows(x).status.item()) == 0
+    H.head_logits(o.out, w, status=word)
+    assert int(word.item()) == 0
+    for bad in (word.float(), word.cpu(), torch.zeros(2, dtype=torch.int32, device=DEV)):
+        with pytest.raises(ValueError, match="status"):
+            H.norm_rows(x, status=bad)
