@@ -45,11 +45,14 @@ DeviceInfo device_info(int* dev_out = nullptr) {
 }
 
 // Raises a kernel's dynamic shared-memory limit on the current device when `smem` exceeds what
-// an earlier launch already asked for; `granted` is the kernel's own per-device record.
+// an earlier launch already asked for; `granted` is the kernel's own per-device record.  Setting and recording are one
+// step to other threads: the limit is the last size set, so that a smaller one set in between would leave the record above it.
 template <class K>
 int ensure_smem(K kern, size_t smem, std::atomic<int>* granted) {
     int dev = -1;
     (void)device_info(&dev);
+    if (dev >= 0 && (size_t)granted[dev].load(std::memory_order_relaxed) >= smem) return 0;
+    std::lock_guard<std::mutex> lock(g_device_mutex);
     if (dev >= 0 && (size_t)granted[dev].load(std::memory_order_relaxed) >= smem) return 0;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return (int)e;
