@@ -23,6 +23,8 @@ from . import native
 _raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 _DTYPES = {torch.float32: native.DTYPE_F32, torch.bfloat16: native.DTYPE_BF16, torch.float8_e4m3fn: native.DTYPE_E4M3}
 
+_INT32_MAX = 2 ** 31 - 1
+
 
 def _check(lib, code, where):
     if code != 0:
@@ -39,6 +41,8 @@ def _rows(t, name, dtypes, device=None, shape=None):
         raise ValueError("%s must be a 2-D CUDA tensor with unit column stride" % name)
     if t.dtype not in dtypes:
         raise ValueError("%s must be %s" % (name, " or ".join(str(d).replace("torch.", "") for d in dtypes)))
+    if max(t.shape) > _INT32_MAX:  # ctypes would keep the low bits
+        raise ValueError("%s has more than %d rows or columns" % (name, _INT32_MAX))
     if device is not None and t.device != device:
         raise ValueError("%s is on %s, not on %s" % (name, t.device, device))
     if shape is not None and tuple(t.shape) != tuple(shape):
