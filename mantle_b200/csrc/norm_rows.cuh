@@ -458,7 +458,7 @@ int launch_norm_as(const NormArgs& a, cudaStream_t stream) {
     // A warp a row, four to a CTA: short rows, and rows of up to 1024 columns where there are many.  (Not where
     // element-wise rows need the CTA's group maxima.)
     if (VEC || !QUANT) {
-        const int grid = (a.rows + 3) / 4;
+        const int grid = (a.rows - 1) / 4 + 1;  // (rows + 3 may pass 2^31)
         if (eights <= 32) return launch_norm_kernel(norm_rows_kernel<T, QUANT, 1, VEC, true>, a, grid, 128, 0, stream);
         if (many && eights <= 64) return launch_norm_kernel(norm_rows_kernel<T, QUANT, 2, VEC, true>, a, grid, 128, 0, stream);
         if (many && eights <= 128) return launch_norm_kernel(norm_rows_kernel<T, QUANT, 4, VEC, true>, a, grid, 128, 0, stream);
