@@ -466,13 +466,19 @@ int launch_norm_as(const NormArgs& a, cudaStream_t stream) {
     if constexpr (VEC) {
         // The ring: where a CTA gets several rows, and a row is worth a bulk copy.  One eight a thread up to 2048
         // columns, two up to 8192 (16 384 x 8192: 193 us with four and 256 threads, 170 with two and 512), four above.
+        // Up to 2048 columns in bfloat16 alone, against a CTA a row: 32 768 x 1280 39 us and 49, 8192 x 1280 with
+        // residual 16.4 and 18.8; not with a residual from some ten thousand rows on (32 768 x 1536: 76 and 70), nor in
+        // float32 (32 768 x 1536: 78 and 61).
         const size_t row = (a.residual ? 2 : 1) * (size_t)a.hidden * sizeof(T), room = (size_t)device_info().per_sm;
         const int vpt = eights <= 256 ? 1 : eights <= 2 * NORM_STREAM_NT ? 2 : 4, threads = ((eights + vpt - 1) / vpt + 31) / 32 * 32;
         // as many CTAs as are resident: 42 registers a thread, 64 with two eights, 128 with four; 2 KB of an SM's room are
         // not theirs
         const int per_sm = (int)std::min<size_t>((size_t)((vpt == 1 ? 1536 : vpt == 2 ? 1024 : 512) / threads), room / (NORM_RING * row + 2048));
-        if (eights >= 256 && eights <= 4 * NORM_STREAM_NT && per_sm >= 1 && a.rows >= 3ll * device_sms() * per_sm) {
-            if (vpt == 1) return launch_norm_stream<T, QUANT, 1>(a, threads, per_sm, NORM_RING * row, stream);
+        const bool worth = vpt > 1 || (sizeof(T) == 2 && eights > 128 && (!a.residual || a.rows <= 16384));
+        if (worth && eights <= 4 * NORM_STREAM_NT && per_sm >= 1 && a.rows >= 3ll * device_sms() * per_sm) {
+            if constexpr (sizeof(T) == 2) {
+                if (vpt == 1) return launch_norm_stream<T, QUANT, 1>(a, threads, per_sm, NORM_RING * row, stream);
+            }
             if (vpt == 2) return launch_norm_stream<T, QUANT, 2>(a, threads, per_sm, NORM_RING * row, stream);
             return launch_norm_stream<T, QUANT, 4>(a, threads, per_sm, NORM_RING * row, stream);
         }
@@ -480,7 +486,7 @@ int launch_norm_as(const NormArgs& a, cudaStream_t stream) {
     // A CTA a row.  Few rows: as few eights a thread as 512 threads allow, the shortest path through the kernel.  Many
     // rows: up to four, more bytes in flight for the same threads.
     int vpt = 1;
-    while (eights > vpt * NORM_NT || (vpt < 4 && many && eights >= vpt * 128)) vpt *= 2;
+    while (eights > vpt * NORM_NT || (vpt < 4 && many && eights > vpt * 128)) vpt *= 2;
     const int threads = ((eights + vpt - 1) / vpt + 31) / 32 * 32;
     if (vpt == 1) return launch_norm_kernel(norm_rows_kernel<T, QUANT, 1, VEC, false>, a, a.rows, threads, 0, stream);
     if (vpt == 2) return launch_norm_kernel(norm_rows_kernel<T, QUANT, 2, VEC, false>, a, a.rows, threads, 0, stream);
