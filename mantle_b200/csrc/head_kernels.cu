@@ -201,14 +201,27 @@ EncodeTiled encode_fn() {
     return f;
 }
 
+// A thread that has made no call of the runtime yet has no current context, and the driver's own calls want one.  (Where one
+// is current, the runtime's or the caller's, it is left alone.)
+bool bind_context() {
+    int dev = 0;
+    return cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess;
+}
+
 // Tiles of `box` from a [d2][d1][d0] array with row strides in bytes; what lies outside reads as zero.
 bool encode(CUtensorMap* m, const void* p, bool eight, int rank, const cuuint64_t* dims, const cuuint64_t* strides,
             const cuuint32_t* box, CUtensorMapSwizzle swizzle) {
     const EncodeTiled f = encode_fn();
     const cuuint32_t steps[3] = {1, 1, 1};
-    return f && f(m, eight ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (cuuint32_t)rank, const_cast<void*>(p),
-                  dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    auto call = [&] {
+        return f(m, eight ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (cuuint32_t)rank, const_cast<void*>(p),
+                 dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    };
+    if (!f) return false;
+    CUresult r = call();
+    if ((r == CUDA_ERROR_INVALID_CONTEXT || r == CUDA_ERROR_NOT_INITIALIZED) && bind_context()) r = call();
+    return r == CUDA_SUCCESS;
 }
 bool encode_rows(CUtensorMap* m, const void* p, bool eight, long long rows, long long cols, long long stride_bytes, int box_rows) {
     const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)stride_bytes};
