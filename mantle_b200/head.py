@@ -11,7 +11,9 @@ adapters of a batch's requests (HeadPlan, Adapters, head_logits).
 
 A plan binds a descriptor to device tensors, as sampler.BatchPlan does: built once, launched many times,
 captured into a CUDA graph where wanted.  It owns its outputs and its workspace, so two plans may run at the
-same time; two launches of one plan may not.  torch supplies device memory and streams; all arithmetic
+same time; two launches of one plan may not.  It may be launched on any stream of its device and dropped at once: its
+memory, and the inputs' that it keeps, is handed out again only when the streams it ran on are done.  (Not so for a
+captured graph, which the caller keeps the plan for.)  torch supplies device memory and streams; all arithmetic
 happens in the CUDA library.
 """
 import ctypes as C
@@ -77,10 +79,30 @@ class _Plan:
         self.device = device
         self._index = device.index
         self.lib = native.load()
+        self._streams = {_raw_stream(self._index)}  # those that the memory below is tied to
+
+    def _own(self, made, given):
+        """What the plan reads and writes: its own tensors, and the caller's, which it keeps alive."""
+        self.keep = given
+        self._memory = [t for t in made + given if t is not None]
+
+    def use_on(self, stream):
+        """Ties the plan's memory to `stream` before it is used there: what is dropped while the stream still runs is not
+        handed out again until it is done.  (Streams that torch does not own may end before the memory does: not those.)"""
+        if stream.cuda_stream not in self._streams:
+            self._tie(stream)
+
+    def _tie(self, stream):
+        self._streams.add(stream.cuda_stream)
+        if not isinstance(stream, torch.cuda.ExternalStream):
+            for t in self._memory:
+                t.record_stream(stream)
 
     def _queue(self, stream):
         # the stream that is current on the plan's device, whatever device is current
         s = _raw_stream(self._index) if stream is None else stream.cuda_stream
+        if s not in self._streams:
+            self.use_on(torch.cuda.current_stream(self._index) if stream is None else stream)
         if _current_device() == self._index:
             rc = self._fn(*self._args, s)
         else:
@@ -88,7 +110,6 @@ class _Plan:
                 rc = self._fn(*self._args, s)
         if rc:
             _check(self.lib, rc, self._name)
-
 
     def check(self):
         """Raises where a wait inside one of the launches so far ran out, whose outputs are then not valid, and clears
@@ -175,7 +196,7 @@ class NormPlan(_Plan):
         b.status = self._status(status)
         self.rows, self.hidden = rows, hidden
         self.out, self.scales, self.residual_out = out, scales, residual_out
-        self.keep = [x, weight, residual]
+        self._own([out, scales, residual_out, self.status], [x, weight, residual])
         self.batch = b
         self._args = (C.byref(b),)
         self._fn, self._name = self.lib.mantleCudaNormRows, "mantleCudaNormRows"
@@ -192,7 +213,10 @@ class NormPlan(_Plan):
 def norm_rows(x, weight=None, stream=None, **kw):
     """One-shot form of NormPlan.  Its outputs carry `status`, which is not 0 where a wait inside the kernel ran out."""
     with torch.cuda.device(x.device), torch.cuda.stream(stream):  # outputs belong to the stream that writes them
-        return NormPlan(x, weight, **kw).launch()
+        plan = NormPlan(x, weight, **kw)
+        if stream is not None:  # made here, but what the caller gave may belong to another
+            plan._tie(stream)
+        return plan.launch()
 
 
 class Adapters:
@@ -326,7 +350,7 @@ class HeadPlan(_Plan):
         self.workspace = torch.empty(n.value, dtype=torch.uint8, device=dev) if n.value else None
         self.kernels_per_launch = c.value
         self.rows, self.vocab, self.out = rows, vocab, out
-        self.keep = reads
+        self._own([out, self.workspace, self.status], reads)
         self.batch = b
         self._args = (C.byref(b), None if self.workspace is None else self.workspace.data_ptr(), n.value)
         self._fn, self._name = self.lib.mantleCudaHeadRows, "mantleCudaHeadRows"
@@ -342,4 +366,6 @@ def head_logits(hidden, weight=None, stream=None, **kw):
     """One-shot form of HeadPlan.  Pass `status` to learn of a wait inside the kernel that ran out."""
     with torch.cuda.device(hidden.device), torch.cuda.stream(stream):
         plan = HeadPlan(hidden, weight, **kw)
+        if stream is not None:
+            plan._tie(stream)
         return plan.launch()

@@ -563,6 +563,9 @@ class BatchSampler:
         u = np.ascontiguousarray(uniforms, dtype=np.float64)
         if u.shape != (self.rows,):
             raise ValueError("one uniform per row")
+        for plan in (head, norm):
+            if plan is not None:
+                plan.use_on(torch.cuda.current_stream(self.device) if stream is None else stream)
         with torch.cuda.device(self.device):
             rc = self.lib.mantleBatchSamplerStepHidden(
                 self.handle, None if norm is None else C.byref(norm.batch), C.byref(head.batch), _ptr(head.workspace),
