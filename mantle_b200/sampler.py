@@ -492,6 +492,8 @@ class BatchSampler:
     def __init__(self, rows, vocab, hist_capacity, stop_tokens=(), device="cuda:0"):
         self.lib = native.load()
         self.device = torch.device(device)
+        if self.device.type == "cuda" and self.device.index is None:  # the device that is current now: its memory lies there
+            self.device = torch.device("cuda", torch.cuda.current_device())
         self.rows, self.vocab = rows, vocab
         stop = np.ascontiguousarray(list(stop_tokens), dtype=np.int64)
         with torch.cuda.device(self.device):
@@ -558,7 +560,7 @@ class BatchSampler:
     def step_hidden_async(self, head, uniforms, norm=None, stream=None, logit_scale=0.0, logit_softcap=0.0):
         """Queues norm (head.NormPlan, optional), head (head.HeadPlan) and one step on the logits it writes."""
         for plan in (head, norm):
-            if plan is not None and self.device.index is not None and plan.device != self.device:
+            if plan is not None and plan.device != self.device:
                 raise ValueError("the plans are not on %s" % self.device)
         u = np.ascontiguousarray(uniforms, dtype=np.float64)
         if u.shape != (self.rows,):

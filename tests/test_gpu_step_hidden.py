@@ -114,3 +114,16 @@ def test_status_words_of_the_one_shot_forms():
     for bad in (word.float(), word.cpu(), torch.zeros(2, dtype=torch.int32, device=DEV)):
         with pytest.raises(ValueError, match="status"):
             H.norm_rows(x, status=bad)
+
+
+def test_a_sampler_without_a_device_number_stays_on_its_device():
+    """"cuda" means the device that is current when the sampler is made, then and later."""
+    by = started(4, 100, device="cuda")
+    assert by.device == torch.device("cuda", torch.cuda.current_device())
+    plan = H.HeadPlan(rand(1, 4, 64).to(BF16), rand(2, 100, 64).to(BF16))
+    other = type("Plan", (), dict(device=torch.device("cuda", 5), batch=plan.batch, workspace=None, workspace_bytes=0,
+                                  use_on=lambda self, stream: None))()
+    with pytest.raises(ValueError, match="not on"):
+        by.step_hidden_async(other, np.zeros(4))
+    by.step_hidden(plan, generators(4))
+    by.close()
