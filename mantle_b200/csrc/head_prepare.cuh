@@ -383,6 +383,15 @@ __global__ void __launch_bounds__(SHRINK_NT) head_shrink_here_kernel(const HeadP
     if (i + (tid >> 4) < n) store_u(p, j0 + (tid & 15), u_row + mine[i + (tid >> 4)], v);
 }
 
+// Two factors as they are packed: an infinity or NaN as the largest finite value.  A step of the tensor cores multiplies
+// every factor of its adapter with the zeros that u has for the other rows of the window, and zero times infinity would
+// reach those.
+__device__ __forceinline__ uint32_t finite_bf16x2(uint32_t two) {
+    if ((two & 0x7f80u) == 0x7f80u) two = (two & 0xffff8000u) | 0x7f7fu;
+    if ((two & 0x7f800000u) == 0x7f800000u) two = (two & 0x8000ffffu) | 0x7f7f0000u;
+    return two;
+}
+
 // B of the adapters as the tensor cores read it, so that any run of 8 vocabulary rows of a chunk of 16 ranks is one
 // contiguous copy: [n][chunks][padded / 8][2][8][8], blocks of 8 vocabulary rows by 8 ranks; zeros behind the
 // vocabulary and the rank.  (From [vocab][rank] rows of 32 bytes the copies ran at a few requests a microsecond: 16
@@ -397,6 +406,7 @@ __global__ void __launch_bounds__(256) adapter_pack_kernel(const bf16_raw* b, in
         const int k = (int)(above % chunks) * U_RANKS + in_group / 8 * 8;
         uint4 w = make_uint4(0, 0, 0, 0);
         if (v < vocab && k < rank) w = *reinterpret_cast<const uint4*>(b + (above / chunks * vocab + v) * rank + k);
+        w = make_uint4(finite_bf16x2(w.x), finite_bf16x2(w.y), finite_bf16x2(w.z), finite_bf16x2(w.w));
         reinterpret_cast<uint4*>(packed)[t] = w;
     }
 }

@@ -224,8 +224,10 @@ class Adapters:
 
     a     [n, rank, hidden] bfloat16     b     [n, vocab, rank] bfloat16, both contiguous
     gain  optional [n] float32 (alpha / rank, usually)
-    rank is a multiple of 8; adapters of smaller rank are padded with zeros.  Everything in a and b is finite.
-    b is copied into the layout the projection reads (on the current stream, once); a and gain are kept as they are.
+    rank is a multiple of 8; adapters of smaller rank are padded with zeros.  Everything in a and b is finite; an
+    adapter that is not spoils the rows that use it, and no others.
+    b is copied into the layout the projection reads (on the current stream, once); a and gain are kept as they are:
+    replace() writes into the caller's own tensors, and what the caller writes there is used from then on.
     """
 
     def __init__(self, a, b, gain=None):
