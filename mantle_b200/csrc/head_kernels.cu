@@ -429,7 +429,7 @@ extern "C" int mantleCudaHeadRows(const MantleHeadBatch* b, void* workspace, siz
     if (l.adapters) {
         const long long per_adapter = (long long)l.chunks * a.b_rows;
         for (int m = 0; m < 4; m++) ok = ok && encode_plain(&maps.b[m], b->adapter_b, per_adapter, b->n_adapters, (VT >> m) / 4);
-        ok = ok && encode_plain(&maps.u, p.u, (long long)l.chunks * l.u_rows / 2, 0, a.u_box / 2);
+        ok = ok && encode_plain(&maps.u, p.u, (long long)l.chunks * l.u_rows / 8 * (8 * U_BYTES / 128), 0, a.u_box / 8 * (8 * U_BYTES / 128));
     }
     if (!ok) return refuse("head: the driver refused a tensor map");
 

@@ -22,7 +22,8 @@ namespace {
 
 constexpr int WINDOW = 32;         // sorted: windows start and end on a multiple of 32 columns of their tile
 constexpr int U_RANKS = 16;        // ranks of one step of the tensor cores: a chunk
-constexpr int U_BYTES = 4 * U_RANKS;  // a row of u of one chunk: sixteen leading parts and sixteen remainders
+constexpr int U_PARTS = 3;         // bfloat16 that hold a value of u: three keep the 24 bits of its float32
+constexpr int U_BYTES = U_PARTS * 2 * U_RANKS;  // a row of u of one chunk
 constexpr int HERE_ROWS = 128;
 constexpr int SORT_NT = 1024;
 constexpr int SHRINK_NT = 512;
@@ -57,7 +58,7 @@ struct HeadPrep {
     HeadBox* boxes;
     int* tile_first;  // [row_tiles + 1] first slot of a tile
     int* n_boxes;     // [1]
-    bf16_raw* u;      // [chunks][u_rows / 8][4][8][8], see u_at
+    bf16_raw* u;      // [chunks][u_rows / 8][U_PARTS * 2][8][8], see u_at
     void* xs;         // [rows][hidden] contiguous, sorted
 };
 
@@ -273,21 +274,24 @@ __device__ __forceinline__ float shrink32(const HeadPrep& p, int adapter, int j0
 }
 
 // u lies in memory as the tensor cores read it from shared memory without swizzle: blocks of 8 rows by 8 values (16
-// bytes a row), four to a group of 8 rows -- leading parts of ranks 0-7 and 8-15 of the chunk, then the remainders --
+// bytes a row), six to a group of 8 rows -- leading parts of ranks 0-7 and 8-15 of the chunk, then second and third parts --
 // so that any run of rows is one contiguous copy.
 __device__ __forceinline__ bf16_raw* u_at(const HeadPrep& p, int rank_at, int u_row) {
     return p.u + ((long long)(rank_at / U_RANKS) * p.u_rows + (u_row & ~7)) * (U_BYTES / 2) +
            (rank_at % U_RANKS / 8) * 64 + (u_row & 7) * 8 + rank_at % 8;
 }
 
-// v in two bfloat16: 16 bits of mantissa (an infinity or NaN stays in the leading part alone).
+// v in three bfloat16, each the rounding of what those before it leave: 24 bits of mantissa, the float32's own (an
+// infinity or NaN stays in the leading part alone).  In two, 16 bits, adapters on a base were off by 4.9e-7 of the
+// logits where float32 sums are by 1.3e-7.
 __device__ __forceinline__ void store_u(const HeadPrep& p, int rank_at, int u_row, float v) {
-    const uint32_t hi = pack_bf16(v, 0.0f) & 0xffffu;
-    const float rest = v - __uint_as_float(hi << 16);
-    const uint32_t lo = (hi & 0x7f80u) == 0x7f80u ? 0u : pack_bf16(rest, 0.0f) & 0xffffu;
     bf16_raw* u = u_at(p, rank_at, u_row);
-    u[0] = (bf16_raw)hi;
-    u[128] = (bf16_raw)lo;
+#pragma unroll
+    for (int i = 0; i < U_PARTS; i++) {
+        const uint32_t part = pack_bf16(v, 0.0f) & 0xffffu;
+        u[128 * i] = (bf16_raw)part;
+        v = (part & 0x7f80u) == 0x7f80u ? 0.0f : v - __uint_as_float(part << 16);
+    }
 }
 
 // Sorted form.  CTAs [0, units) x [0, chunks): one chunk of ranks of one box.  CTAs from `units` on: the copy of x.
