@@ -186,7 +186,7 @@ func AdapterPack(b DeviceBuffer, n, vocab, rank int, packed DeviceBuffer, stream
 
 // StepHidden queues norm (nil: none), head and one sampling step on the logits that the head writes.
 func (s *BatchSampler) StepHidden(norm *NormBatch, head *HeadBatch, workspace DeviceBuffer, uniforms []float64, post HeadPost, stream Stream) error {
-	if head == nil || len(uniforms) != s.rows {
+	if head == nil || len(uniforms) == 0 || len(uniforms) != s.rows {
 		return fmt.Errorf("batch sampler step: nil head or %d uniforms for %d rows", len(uniforms), s.rows)
 	}
 	ch := head.c()

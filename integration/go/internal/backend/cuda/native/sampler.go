@@ -631,7 +631,7 @@ func (s *BatchSampler) CanUseDeviceGreedy(row int) bool {
 
 // Step queues one step for every live row; uniforms holds one draw per row.
 func (s *BatchSampler) Step(logits DeviceBuffer, bf16 bool, rowStride int64, uniforms []float64, post HeadPost, stream Stream) error {
-	if logits.ptr == nil || len(uniforms) != s.rows {
+	if logits.ptr == nil || len(uniforms) == 0 || len(uniforms) != s.rows {
 		return fmt.Errorf("batch sampler step: nil logits or %d uniforms for %d rows", len(uniforms), s.rows)
 	}
 	dtype := C.int(0)
