@@ -265,6 +265,8 @@ class Adapters:
                 raise ValueError("%s must be a contiguous %s bfloat16 tensor on %s" % (name, shape, self.device))
         if b.data_ptr() % 16:
             raise ValueError("b must start on 16 bytes")
+        if gain is not None and not (isinstance(gain, torch.Tensor) and gain.dim() == 0):
+            gain = float(gain)  # what is no number is refused before anything is written
         self.a[i].copy_(a)
         if gain is not None:
             self.gain[i].fill_(gain)

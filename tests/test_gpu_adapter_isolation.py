@@ -35,3 +35,15 @@ def test_an_adapter_that_is_not_finite_spoils_its_own_rows_only(rows, dtype, bes
                 assert torch.equal(got[keep], clean[keep]), (value, where, replaced)
                 if bool((~keep).any()):
                     assert not torch.equal(got[~keep], clean[~keep])
+
+
+@pytest.mark.parametrize("gain", ["much", None, [1.0, 2.0], torch.ones(2)])
+def test_a_refused_replacement_leaves_the_table_as_it_was(gain):
+    s = head_inputs(10, 300, 128, BF16, 3, 8)
+    t = head_inputs(10, 300, 128, BF16, 3, 8, seed=40)
+    table = H.Adapters(s["a"], s["b"], s["gain"])
+    kept = [x.clone() for x in (table.a, table.gain, table.packed)]
+    with pytest.raises((TypeError, ValueError)):
+        table.replace(1, t["a"][0], t["b"][0], gain)
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(kept, (table.a, table.gain, table.packed)))
