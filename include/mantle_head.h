@@ -111,10 +111,10 @@ int mantleCudaNormRows(const MantleNormBatch* batch, mantleCudaStream_t stream);
  *   status       optional: one int32 that MANTLE_SAMPLE_STATUS_TIMEOUT is OR-ed into when a wait inside the
  *                kernel ran out (two seconds; the output is then not valid)
  *
- * Sums are float32, and between the adapter's two products a value keeps its 24 bits.  The factors of an adapter
- * have to be finite: an infinity or NaN in its `b` is packed as the largest finite value (rows of several adapters share
- * a step of the tensor cores, where an infinity times another row's zero would be NaN), so that what is not finite
- * spoils the rows that use the adapter, and no others.
+ * Sums are float32; between the adapter's two products a value keeps its 24 bits (16 where the logits are bfloat16, of
+ * 8 bits themselves).  The factors of an adapter have to be finite: an infinity or NaN in its `b` is packed as the largest
+ * finite value (rows of several adapters share a step of the tensor cores, where an infinity times another row's zero
+ * would be NaN), so that what is not finite spoils the rows that use the adapter, and no others.
  *
  * `workspace`: mantleCudaHeadWorkspaceBytes() bytes on 256 bytes, needed with adapters or where hidden_rows do
  * not start on 16 bytes each, else NULL is fine.  Its contents mean nothing between calls; two calls that may

@@ -124,7 +124,7 @@ struct HeadLayout {
     bool sorted;  // rows in the order of their adapters
     bool copied;  // x is read from the workspace's copy
     bool pair;    // two CTAs to a tile
-    int tile_cols, row_tiles, v_tiles, w_steps, chunks, slot_bound, box_bound, u_rows;
+    int tile_cols, row_tiles, v_tiles, w_steps, chunks, slot_bound, box_bound, u_rows, parts;
     int stages, stage_bytes, grid;
     size_t smem;
     size_t perm, slots, boxes, tile_first, n_boxes, u, xs, total;
@@ -163,6 +163,7 @@ HeadLayout head_layout(const MantleHeadBatch* b) {
     };
     if (l.adapters) {
         l.chunks = (b->rank + U_RANKS - 1) / U_RANKS;
+        l.parts = u_parts(b->out_dtype == MANTLE_DTYPE_BF16);
         l.slot_bound = std::min(b->rows, b->n_adapters);
         if (l.sorted) {
             // a piece per adapter in use and one per tile's end; each box holds a row at least, and a piece of n rows
@@ -176,7 +177,7 @@ HeadLayout head_layout(const MantleHeadBatch* b) {
         l.u_rows = l.sorted ? l.box_bound * WINDOW : l.slot_bound * l.tile_cols;
         l.slots = take((size_t)l.slot_bound * sizeof(HeadSlot));
         l.tile_first = take((size_t)(l.row_tiles + 1) * 4);
-        l.u = take((size_t)l.chunks * (size_t)l.u_rows * U_BYTES);
+        l.u = take((size_t)l.chunks * (size_t)l.u_rows * u_bytes(l.parts));
     }
     if (l.copied) l.xs = take((size_t)b->rows * (size_t)b->hidden * e);
     return l;
@@ -373,7 +374,7 @@ extern "C" int mantleCudaHeadRows(const MantleHeadBatch* b, void* workspace, siz
     a.b_rows = padded / 4;
     a.stages = l.stages;
     a.stage_bytes = l.stage_bytes;
-    a.pack_bytes = B_BYTES + l.tile_cols / (l.pair ? 2 : 1) * U_BYTES;
+    a.pack_bytes = B_BYTES + l.tile_cols / (l.pair ? 2 : 1) * u_bytes(l.parts);
     a.pack = l.stage_bytes / a.pack_bytes;
     a.x_scales = b->hidden_scales;
     a.w_scales = b->weight_scales;
@@ -397,6 +398,7 @@ extern "C" int mantleCudaHeadRows(const MantleHeadBatch* b, void* workspace, siz
     p.n_adapters = b->n_adapters;
     p.rank = b->rank;
     p.u_rows = l.u_rows;
+    p.parts = l.parts;
     p.tile_cols = l.tile_cols;
     p.row_tiles = l.row_tiles;
     p.units = l.sorted ? l.box_bound : l.slot_bound;
@@ -429,7 +431,7 @@ extern "C" int mantleCudaHeadRows(const MantleHeadBatch* b, void* workspace, siz
     if (l.adapters) {
         const long long per_adapter = (long long)l.chunks * a.b_rows;
         for (int m = 0; m < 4; m++) ok = ok && encode_plain(&maps.b[m], b->adapter_b, per_adapter, b->n_adapters, (VT >> m) / 4);
-        ok = ok && encode_plain(&maps.u, p.u, (long long)l.chunks * l.u_rows / 8 * (8 * U_BYTES / 128), 0, a.u_box / 8 * (8 * U_BYTES / 128));
+        ok = ok && encode_plain(&maps.u, p.u, (long long)l.chunks * u_lines(l.u_rows, l.parts), 0, u_lines(a.u_box, l.parts));
     }
     if (!ok) return refuse("head: the driver refused a tensor map");
 

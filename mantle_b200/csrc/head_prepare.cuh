@@ -22,8 +22,12 @@ namespace {
 
 constexpr int WINDOW = 32;         // sorted: windows start and end on a multiple of 32 columns of their tile
 constexpr int U_RANKS = 16;        // ranks of one step of the tensor cores: a chunk
-constexpr int U_PARTS = 3;         // bfloat16 that hold a value of u: three keep the 24 bits of its float32
-constexpr int U_BYTES = U_PARTS * 2 * U_RANKS;  // a row of u of one chunk
+// Bfloat16 that hold a value of u, side by side.  Three keep the 24 bits of its float32; two keep 16, which adds a
+// 256th to what the rounding of bfloat16 logits takes.
+__host__ __device__ constexpr int u_parts(bool out16) { return out16 ? 2 : 3; }
+__host__ __device__ constexpr int u_bytes(int parts) { return parts * 2 * U_RANKS; }  // a row of u of one chunk
+// That many rows of u, whole eights, in rows of 128 bytes, as tensor maps count them.
+__host__ __device__ constexpr int u_lines(int rows, int parts) { return rows / 8 * (8 * u_bytes(parts) / 128); }
 constexpr int HERE_ROWS = 128;
 constexpr int SORT_NT = 1024;
 constexpr int SHRINK_NT = 512;
@@ -49,7 +53,7 @@ struct HeadPrep {
     long long x_stride;  // elements
     int rows, hidden, e4m3, vec;  // vec: rows of x start on 16 bytes
     int n_adapters, rank;
-    int u_rows;          // rows of u of one chunk of ranks
+    int u_rows, parts;   // rows of u of one chunk of ranks; see u_parts
     int tile_cols, row_tiles;
     int units, copy_ctas;  // CTAs of the shrink kernel: slots or boxes at most; and those that copy x
     // workspace
@@ -58,7 +62,7 @@ struct HeadPrep {
     HeadBox* boxes;
     int* tile_first;  // [row_tiles + 1] first slot of a tile
     int* n_boxes;     // [1]
-    bf16_raw* u;      // [chunks][u_rows / 8][U_PARTS * 2][8][8], see u_at
+    bf16_raw* u;      // [chunks][u_rows / 8][parts * 2][8][8], see u_at
     void* xs;         // [rows][hidden] contiguous, sorted
 };
 
@@ -274,20 +278,19 @@ __device__ __forceinline__ float shrink32(const HeadPrep& p, int adapter, int j0
 }
 
 // u lies in memory as the tensor cores read it from shared memory without swizzle: blocks of 8 rows by 8 values (16
-// bytes a row), six to a group of 8 rows -- leading parts of ranks 0-7 and 8-15 of the chunk, then second and third parts --
+// bytes a row), two for each part to a group of 8 rows -- leading parts of ranks 0-7 and 8-15 of the chunk, then the next --
 // so that any run of rows is one contiguous copy.
 __device__ __forceinline__ bf16_raw* u_at(const HeadPrep& p, int rank_at, int u_row) {
-    return p.u + ((long long)(rank_at / U_RANKS) * p.u_rows + (u_row & ~7)) * (U_BYTES / 2) +
+    return p.u + ((long long)(rank_at / U_RANKS) * p.u_rows + (u_row & ~7)) * (u_bytes(p.parts) / 2) +
            (rank_at % U_RANKS / 8) * 64 + (u_row & 7) * 8 + rank_at % 8;
 }
 
-// v in three bfloat16, each the rounding of what those before it leave: 24 bits of mantissa, the float32's own (an
-// infinity or NaN stays in the leading part alone).  In two, 16 bits, adapters on a base were off by 4.9e-7 of the
-// logits where float32 sums are by 1.3e-7.
+// v in its parts, each the rounding of what those before it leave (an infinity or NaN stays in the leading part alone).
+// In two, float32 logits of adapters on a base were off by 4.9e-7 of their size where float32 sums are by 1.3e-7; in
+// three by 1.0e-7.
 __device__ __forceinline__ void store_u(const HeadPrep& p, int rank_at, int u_row, float v) {
     bf16_raw* u = u_at(p, rank_at, u_row);
-#pragma unroll
-    for (int i = 0; i < U_PARTS; i++) {
+    for (int i = 0; i < p.parts; i++) {
         const uint32_t part = pack_bf16(v, 0.0f) & 0xffffu;
         u[128 * i] = (bf16_raw)part;
         v = (part & 0x7f80u) == 0x7f80u ? 0.0f : v - __uint_as_float(part << 16);

@@ -33,9 +33,9 @@
 // columns) and take 4096 rows of 151 936 x 1024 from 1232 to 1666 us; and one length for every batch keeps a row's bits
 // the same in all of them.
 //
-// u comes as three bfloat16 side by side, its parts of 8 bits each: three products with the same B cost no more of its
-// bytes and keep the 24 bits of float32 (64 rows with 16 adapters: 92 us, 86 with two parts and 16 bits).  With 8-bit
-// operands the projection's rounds are scaled by row and column, and the adapters have a round of their own.
+// u comes as bfloat16 side by side, its parts of 8 bits each: three products with the same B cost no more of its bytes
+// and keep the 24 bits of float32 (64 rows with 16 adapters: 92 us, 86 with two parts and 16 bits).  Bfloat16 logits take
+// two.  With 8-bit operands the projection's rounds are scaled by row and column, and the adapters have a round of their own.
 #pragma once
 
 namespace {
@@ -143,7 +143,8 @@ __device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* map, int
 // `group` bytes from eight rows to the next eight.
 // (As two words: the low one holds the address and the distance of blocks, the high one all that does not change.)
 constexpr uint32_t SWIZZLED_ROWS_LO = 1u << 16, SWIZZLED_ROWS_HI = 1024u >> 4 | 1u << 14 | 2u << 29;
-constexpr uint32_t BLOCKS_LO = 128u >> 4 << 16, B_BLOCKS_HI = 256u >> 4 | 1u << 14, U_BLOCKS_HI = 8u * U_BYTES >> 4 | 1u << 14;
+constexpr uint32_t BLOCKS_LO = 128u >> 4 << 16, B_BLOCKS_HI = 256u >> 4 | 1u << 14;
+__device__ constexpr uint32_t u_blocks_hi(int parts) { return 8u * u_bytes(parts) >> 4 | 1u << 14; }
 __device__ __forceinline__ uint32_t operand_lo(uint32_t format, uint32_t addr) { return format | ((addr >> 4) & 0x3fff); }
 // Instruction descriptor: float32 accumulator, 128 (a pair: 256) x n; bfloat16 operands, or e4m3.
 template <bool PAIR>
@@ -299,6 +300,8 @@ __global__ void __launch_bounds__(HEAD_NT, 1) head_rows_kernel(const HeadArgs a,
     constexpr int STEP_COLS = E4M3 ? STEP_BYTES : STEP_BYTES / 2;
     constexpr int ROUND = E4M3 ? ROUND_E4M3 : ROUND_BF16;
     constexpr int OUT_BYTES = OUT16 ? 2 : 4;
+    constexpr int PARTS = u_parts(OUT16), U_BYTES = u_bytes(PARTS);
+    constexpr uint32_t U_BLOCKS_HI = u_blocks_hi(PARTS);
     using Out = typename OutType<OUT16>::type;
     constexpr bool PAIR = GROUPS >= 4;
     constexpr int CTAS = PAIR ? 2 : 1;
@@ -448,7 +451,7 @@ __global__ void __launch_bounds__(HEAD_NT, 1) head_rows_kernel(const HeadArgs a,
                         mbar_expect_more_on(full0 + 8 * stage, (uint32_t)(u_n * U_BYTES * CTAS), on_lead);
 #pragma unroll 1
                         for (int r = 0; r < u_n; r += a.u_box)  // eight rows of u to a whole number of 128 bytes
-                            tma_2d<PAIR>(to + B_BYTES + r * U_BYTES, &maps.u, 0, (step.z + half * u_n + r) / 8 * (8 * U_BYTES / 128), bar, on);
+                            tma_2d<PAIR>(to + B_BYTES + r * U_BYTES, &maps.u, 0, u_lines(step.z + half * u_n + r, PARTS), bar, on);
                     }
                     to += (uint32_t)a.pack_bytes;
                     if (++place == a.pack || i == n - 1) {
@@ -547,7 +550,7 @@ __global__ void __launch_bounds__(HEAD_NT, 1) head_rows_kernel(const HeadArgs a,
                         const uint32_t d = acc + (uint32_t)(window & 0xffff), n_shape = shape_bf16<PAIR>(window >> 16);
                         const uint32_t b_lo = operand_lo(BLOCKS_LO, at), u_lo = operand_lo(BLOCKS_LO, at + B_BYTES);
 #pragma unroll
-                        for (int part = 0; part < U_PARTS; part++)
+                        for (int part = 0; part < PARTS; part++)
                             mma<PAIR, false>(d, b_lo, B_BLOCKS_HI, u_lo + part * (256 >> 4), U_BLOCKS_HI, n_shape, true, on);
                         at += (uint32_t)a.pack_bytes;
                         if (++place == a.pack || i == n - 1) {
