@@ -12,10 +12,11 @@
 // nothing.
 //
 // Two forms.  Up to HERE_ROWS rows, one kernel: rows stay where they are, and an adapter's window is the whole
-// tile, zeros and all; the projection can then read x and W from its first cycle on, and meets this kernel's
-// results only when it comes to the adapters.  More rows: head_sort_kernel puts the rows in an order in which
-// those of one adapter stand together, and head_shrink_kernel copies x in that order, so that a window covers an
-// adapter's own rows and little else.
+// tile, zeros and all; the projection does not wait for this kernel before it reads x and W, and meets its results only
+// when it comes to the adapters.  (It starts at once on the SMs that have no CTA of this kernel: the two do not fit on
+// one SM together, 34 KB here beside a ring that fills the rest.)  More rows: head_sort_kernel puts the rows in an
+// order in which those of one adapter stand together, and head_shrink_kernel copies x in that order, so that a window
+// covers an adapter's own rows and little else.
 #pragma once
 
 namespace {

@@ -34,7 +34,7 @@
 // the same in all of them.
 //
 // u comes as bfloat16 side by side, its parts of 8 bits each: three products with the same B cost no more of its bytes
-// and keep the 24 bits of float32 (64 rows with 16 adapters: 92 us, 86 with two parts and 16 bits).  Bfloat16 logits take
+// and keep the 24 bits of float32 (64 rows with 16 adapters: 90 us, 85 with two parts and 16 bits).  Bfloat16 logits take
 // two.  With 8-bit operands the projection's rounds are scaled by row and column, and the adapters have a round of their own.
 #pragma once
 

@@ -352,11 +352,12 @@ __global__ void __launch_bounds__(WARP_ROW ? 128 : NORM_NT) norm_rows_kernel(con
     norm_finish<T, QUANT, VPT, VEC, WARP_ROW>(a, row, c, s, weight, part, group_max, [] {});
 }
 
-// Many long rows: CTAs that stay, each with a ring of rows of x and residual in shared memory that bulk copies fill ahead.  In registers alone an SM holds no more bytes in flight than its threads have room for beside the row they
-// work on, and none at all between a CTA's end and the next one's first load (16 384 x 8192 bfloat16 with residual, to
-// 8 bits: 243 us so, 150 here, 97 % of the measured copy bandwidth).  The row's factors stay in registers as they
-// are used: with them packed, and a test for the row's end at every value, instruction issue was the bound (36
-// instructions a value, 170 us).
+// Many long rows: CTAs that stay, each with a ring of rows of x and residual in shared memory that bulk copies fill ahead.
+// In registers alone an SM holds no more bytes in flight than its threads have room for beside the row they work on,
+// and none at all between a CTA's end and the next one's first load (16 384 x 8192 bfloat16 with residual, to 8 bits:
+// 243 us so; here 148 at 1965 MHz, 99 % of the measured copy bandwidth, and 167 after a second or two, when the card's
+// 1000 W hold the clock at 1730 MHz).  The row's factors stay in registers as they are used: with them packed, and a
+// test for the row's end at every value, instruction issue was the bound (36 instructions a value, 170 us).
 constexpr int NORM_RING = 2;          // (four deep measured the same)
 constexpr int NORM_STREAM_NT = 512;  // threads at most
 
@@ -471,8 +472,8 @@ int launch_norm_as(const NormArgs& a, cudaStream_t stream) {
         // float32 (32 768 x 1536: 78 and 61).
         const size_t row = (a.residual ? 2 : 1) * (size_t)a.hidden * sizeof(T), room = (size_t)device_info().per_sm;
         const int vpt = eights <= 256 ? 1 : eights <= 2 * NORM_STREAM_NT ? 2 : 4, threads = ((eights + vpt - 1) / vpt + 31) / 32 * 32;
-        // as many CTAs as are resident: 42 registers a thread, 64 with two eights, 128 with four; 2 KB of an SM's room are
-        // not theirs
+        // as many CTAs as are resident: up to 42 registers a thread, 64 with two eights, 128 with four; 2 KB of an SM's
+        // room are not theirs
         const int per_sm = (int)std::min<size_t>((size_t)((vpt == 1 ? 1536 : vpt == 2 ? 1024 : 512) / threads), room / (NORM_RING * row + 2048));
         const bool worth = vpt > 1 || (sizeof(T) == 2 && eights > 128 && (!a.residual || a.rows <= 16384));
         if (worth && eights <= 4 * NORM_STREAM_NT && per_sm >= 1 && a.rows >= 3ll * device_sms() * per_sm) {

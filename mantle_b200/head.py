@@ -141,7 +141,10 @@ class NormPlan(_Plan):
     residual     optional, like x; residual_out receives s rounded to x's type (made here unless given; x or
                  residual themselves may be given)
     out_dtype    None: x's type (out may be x itself).  torch.float8_e4m3fn: 8 bits, `scales` [rows, 1] float32 for
-                 scale_group 0, [rows, ceil(hidden / 128)] for scale_group 128; value = out * scale
+                 scale_group 0, [rows, ceil(hidden / 128)] for scale_group 128; value = out * scale.  HeadPlan reads
+                 scale_group 0; groups are for a reader of the caller's
+    out, scales, residual_out   made here unless given.  Apart from what is said above, nothing that is written may
+                 overlap anything else, by the spans of the tensors: interleaved columns of one buffer count as overlapping
     status       optional [1] int32 on the device, made here unless given: not 0 once a wait inside a launch has run out
                  (check() says so; several plans may share one)
     """
@@ -282,7 +285,7 @@ class HeadPlan(_Plan):
     base           instead of weight: [rows, vocab] of out_dtype, to which the adapters' part is added (out may be base)
     adapters, adapter_ids   a table and the [rows] int32 ids of the requests' adapters; an id outside the table: none
     out_dtype      float32 or bfloat16
-    status         as in NormPlan
+    out, status    as in NormPlan
     """
 
     def __init__(self, hidden, weight=None, hidden_scales=None, weight_scales=None, adapters=None, adapter_ids=None,
