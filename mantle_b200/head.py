@@ -13,7 +13,8 @@ A plan binds a descriptor to device tensors, as sampler.BatchPlan does: built on
 captured into a CUDA graph where wanted.  It owns its outputs and its workspace, so two plans may run at the
 same time; two launches of one plan may not.  It may be launched on any stream of its device and dropped at once: its
 memory, and the inputs' that it keeps, is handed out again only when the streams it ran on are done.  (Not so for a
-captured graph, which the caller keeps the plan for.)  torch supplies device memory and streams; all arithmetic
+captured graph, which the caller keeps the plan for.)  A stream other than the one that made the plan and its inputs
+waits for that one first, as with any kernel: the caller orders them.  torch supplies device memory and streams; all arithmetic
 happens in the CUDA library.
 """
 import ctypes as C
